@@ -1043,6 +1043,76 @@ int pv2_voxelize_stage2(int64_t n, int64_t n_vox, const uint64_t* uniq_keys, con
                         int32_t* members, int32_t* max_count, void* workspace, size_t workspace_bytes,
                         int64_t* idx_unique, int64_t* grid_coord, pv2_stream_t stream);
 
+/* ---- Rows by id (csrc/row_groups.hip) --------------------------------------------------------------------------
+ * The stable order of n rows by an integer id: order [n] lists the rows of id 0 in row order, then those of id 1, ..;
+ * rows whose id is outside 0 .. n_groups - 1 come last.  The rows of id g are order[offsets[g]] .. order[offsets[g+1] - 1]
+ * (offsets [n_groups + 1]).  index: int64 if index_is_64, else int32.  sorted_ids (may be null) [n]: the ids in that
+ * order, n_groups for the rows of no group.  workspace: pv2_row_groups_workspace_ints(n, n_groups) ints.
+ * n < 2^31 - 4096, n_groups <= 2^30.
+ * pv2_row_offsets: the same offsets for rows that already lie group by group, from the groups' cumulative row counts
+ * [n_groups]; whatever the counts hold, the offsets never decrease and lie within 0 .. n. */
+int64_t pv2_row_groups_workspace_ints(int64_t n, int64_t n_groups);
+int pv2_row_groups(const void* index, int index_is_64, int64_t n, int64_t n_groups, int32_t* order, int32_t* offsets,
+                   int32_t* sorted_ids, int32_t* workspace, pv2_stream_t stream);
+int pv2_row_offsets(const void* cumulative, int is_64, int64_t n_groups, int64_t n, int32_t* offsets,
+                    pv2_stream_t stream);
+
+/* ---- Embedding (csrc/embedding.hip) ----------------------------------------------------------------------------
+ * out [n, c] = scale * weight[index[i]], zeros where the index is outside 0 .. rows - 1; weight [rows, c] with
+ * `row_stride` elements between rows; out is contiguous and of the weight's type (PV2_F32 / PV2_BF16 / PV2_F16).
+ * Backward: grad_weight [rows, c] (contiguous, every element written, of the same type) = scale * the sum of the rows
+ * of grad_out whose index it is, in a fixed order, in fp32, rounded once.  workspace: 32-byte aligned,
+ * pv2_embedding_backward_workspace_ints(n, rows, c) ints. */
+int pv2_embedding_forward(const void* index, int index_is_64, int64_t n, const void* weight, int dtype, int64_t rows,
+                          int c, int64_t row_stride, float scale, void* out, pv2_stream_t stream);
+int64_t pv2_embedding_backward_workspace_ints(int64_t n, int64_t rows, int c);
+int pv2_embedding_backward(const void* index, int index_is_64, int64_t n, const void* grad_out, int dtype, int64_t rows,
+                           int c, int64_t grad_row_stride, float scale, int32_t* workspace, void* grad_weight,
+                           pv2_stream_t stream);
+
+/* ---- Linear layers with weights per group of rows (csrc/grouped_linear.hip) -------------------------------------
+ * order / offsets as pv2_row_groups writes them (order null: the rows lie group by group); weight [groups, n_out, n_in]
+ * with the given strides (elements; n_in contiguous), x [rows, n_in] and grad_out [rows, n_out] with a row stride,
+ * everything else contiguous; all of one type (PV2_F32 / PV2_BF16 / PV2_F16), accumulated in fp32.
+ *   forward      out [rows, n_out] = x W_g^T + b_g;   grad_input  grad_x [rows, n_in] = grad_out W_g;
+ *                rows of no group are zeros in both
+ *   grad_weight  grad_weight [groups, n_out, n_in] = grad_out_g^T x_g, grad_bias [groups, n_out] = sum of grad_out_g;
+ *                every element written; workspace: pv2_grouped_linear_workspace_floats (may be null if that is 0). */
+int pv2_grouped_linear_forward(const void* x, int dtype, int64_t rows, int n_in, int64_t x_stride, const void* weight,
+                               int64_t weight_group_stride, int64_t weight_row_stride, int64_t groups, int n_out,
+                               const void* bias_or_null, const int32_t* order_or_null, const int32_t* offsets,
+                               void* out, pv2_stream_t stream);
+int pv2_grouped_linear_grad_input(const void* grad_out, int dtype, int64_t rows, int n_out, int64_t grad_stride,
+                                  const void* weight, int64_t weight_group_stride, int64_t weight_row_stride,
+                                  int64_t groups, int n_in, const int32_t* order_or_null, const int32_t* offsets,
+                                  void* grad_x, pv2_stream_t stream);
+int64_t pv2_grouped_linear_workspace_floats(int64_t rows, int64_t groups, int n_out, int n_in);
+int pv2_grouped_linear_grad_weight(const void* grad_out, int dtype, int64_t rows, int n_out, int64_t grad_stride,
+                                   const void* x, int n_in, int64_t x_stride, int64_t groups,
+                                   const int32_t* order_or_null, const int32_t* offsets, float* workspace,
+                                   void* grad_weight, void* grad_bias_or_null, pv2_stream_t stream);
+
+/* ---- Distillation from a teacher's top logits (csrc/distillation.hip) -------------------------------------------
+ * Row i: p = softmax(teacher_logits[i] / T) over its listed classes (teacher_index[i], k of them; an entry counts if its
+ * class is in 0 .. classes - 1 and its logit above -inf), q = softmax(logits[i] / T); loss_i = T^2 sum p (log p - log q).
+ * A row without an entry that counts has loss 0 and gradient 0.
+ *   forward   loss [1]: the sum of the losses, or with `mean` their mean over the rows that count; count [1]: the number of
+ *             those rows; row_loss [rows] (may be null); stats [rows, 2] for the backward pass
+ *   backward  grad_logits [rows, classes] (contiguous, logits' type) = upstream (one value, or one per row) * d loss_i;
+ *             count_or_null: the forward pass's, where it took the mean
+ * Strides are in elements, the last axis is contiguous; 1 <= k <= 1024. */
+int64_t pv2_topk_distill_workspace_floats(int64_t rows, int classes, int k);
+int pv2_topk_distill_forward(const void* logits, int dtype, int64_t rows, int classes, int64_t row_stride,
+                             const void* teacher_index, int index_is_64, int64_t index_stride,
+                             const void* teacher_logits, int teacher_dtype, int64_t teacher_stride, int k,
+                             float temperature, int mean, float* workspace, float* stats, float* row_loss_or_null,
+                             float* loss, float* count, pv2_stream_t stream);
+int pv2_topk_distill_backward(const void* logits, int dtype, int64_t rows, int classes, int64_t row_stride,
+                              const void* teacher_index, int index_is_64, int64_t index_stride,
+                              const void* teacher_logits, int teacher_dtype, int64_t teacher_stride, int k,
+                              float temperature, const float* stats, const float* upstream, int upstream_per_row,
+                              const float* count_or_null, void* grad_logits, pv2_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

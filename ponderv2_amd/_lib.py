@@ -250,6 +250,29 @@ SIGNATURES["pv2_voxelize_workspace_bytes"] = (c_size_t, [c_int64])
 SIGNATURES["pv2_voxelize_stage2"] = (
     c_int, [c_int64, c_int64] + [_P] * 14 + [_P, c_size_t, _P, _P, _P])
 
+SIGNATURES["pv2_row_groups_workspace_ints"] = (c_int64, [c_int64, c_int64])
+SIGNATURES["pv2_row_groups"] = (c_int, [_P, c_int, c_int64, c_int64, _P, _P, _P, _P, _P])
+SIGNATURES["pv2_row_offsets"] = (c_int, [_P, c_int, c_int64, c_int64, _P, _P])
+SIGNATURES["pv2_embedding_forward"] = (
+    c_int, [_P, c_int, c_int64, _P, c_int, c_int64, c_int, c_int64, c_float, _P, _P])
+SIGNATURES["pv2_embedding_backward_workspace_ints"] = (c_int64, [c_int64, c_int64, c_int])
+SIGNATURES["pv2_embedding_backward"] = (
+    c_int, [_P, c_int, c_int64, _P, c_int, c_int64, c_int, c_int64, c_float, _P, _P, _P])
+SIGNATURES["pv2_grouped_linear_forward"] = (
+    c_int, [_P, c_int, c_int64, c_int, c_int64, _P, c_int64, c_int64, c_int64, c_int, _P, _P, _P, _P, _P])
+SIGNATURES["pv2_grouped_linear_grad_input"] = (
+    c_int, [_P, c_int, c_int64, c_int, c_int64, _P, c_int64, c_int64, c_int64, c_int, _P, _P, _P, _P])
+SIGNATURES["pv2_grouped_linear_workspace_floats"] = (c_int64, [c_int64, c_int64, c_int, c_int])
+SIGNATURES["pv2_grouped_linear_grad_weight"] = (
+    c_int, [_P, c_int, c_int64, c_int, c_int64, _P, c_int, c_int64, c_int64, _P, _P, _P, _P, _P, _P])
+SIGNATURES["pv2_topk_distill_workspace_floats"] = (c_int64, [c_int64, c_int, c_int])
+SIGNATURES["pv2_topk_distill_forward"] = (
+    c_int, [_P, c_int, c_int64, c_int, c_int64, _P, c_int, c_int64, _P, c_int, c_int64, c_int, c_float, c_int,
+            _P, _P, _P, _P, _P, _P])
+SIGNATURES["pv2_topk_distill_backward"] = (
+    c_int, [_P, c_int, c_int64, c_int, c_int64, _P, c_int, c_int64, _P, c_int, c_int64, c_int, c_float,
+            _P, _P, c_int, _P, _P, _P])
+
 _lib = None
 
 

@@ -1,0 +1,352 @@
+// Rows by id: the stable order of n rows by an integer id and the offset of every id's rows in it - what the gradient
+// of an embedding (embedding.hip) and the products with per-group weights (grouped_linear.hip) need.
+//
+// A stable radix sort, least significant digit first, of key(i) = id if 0 <= id < G, else G (so rows without a group
+// come last, in row order).  Digits of up to 10 bits: one pass for G < 1024, two up to 2^20.  A pass is
+//   count    every block's histogram of its 4096 keys (LDS counters),
+//   scan     one block per digit over the blocks' counts,
+//   scatter  every wave walks its 1024 keys in order, 64 at a time; lanes with equal digits find each other by one
+//            ballot per digit bit, and a lane's place is (start of the digit) + (earlier blocks, waves and rounds) +
+//            (equal lanes below it).
+// Nothing depends on the order in which blocks or atomics run.  Up to 4096 rows one workgroup does all passes in LDS
+// in a single launch.
+#include "common.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kTile = 4096;        // keys per block of the multi-block sort
+constexpr int kMaxBits = 10;
+constexpr int kMaxDigits = 1 << kMaxBits;
+constexpr int kSmall = 4096;       // rows that one workgroup sorts in LDS
+constexpr int kSmallThreads = 1024;
+constexpr int kSmallBits = 8;
+
+__device__ __forceinline__ int key_of(const void* index, int is64, int64_t i, int n_groups) {
+  const int64_t id = is64 ? ((const int64_t*)index)[i] : (int64_t)((const int32_t*)index)[i];
+  return (id >= 0 && id < n_groups) ? (int)id : n_groups;
+}
+
+// lanes of `active` that hold the same digit as this one
+__device__ __forceinline__ uint64_t same_digit(int digit, int bits, uint64_t active) {
+  uint64_t m = active;
+  for (int b = 0; b < bits; ++b) {
+    const uint64_t set = __ballot((digit >> b) & 1);
+    m &= ((digit >> b) & 1) ? set : ~set;
+  }
+  return m;
+}
+
+__device__ __forceinline__ int wave_inclusive_scan(int v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int t = __shfl_up(v, d);
+    if (lane >= d) v += t;
+  }
+  return v;
+}
+
+// exclusive scan over the block's threads; *total: the sum
+template <int THREADS>
+__device__ __forceinline__ int block_exclusive_scan(int v, int* s_wave, int* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int inc = wave_inclusive_scan(v);
+  __syncthreads();
+  if (lane == 63) s_wave[wave] = inc;
+  __syncthreads();
+  int before = 0, sum = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    if (w < wave) before += s_wave[w];
+    sum += s_wave[w];
+  }
+  *total = sum;
+  return before + inc - v;
+}
+
+struct Source {      // keys of a pass: the caller's ids (first pass) or the previous pass's keys
+  const void* index;
+  int is64;
+  const int32_t* keys;
+  int n_groups;
+  __device__ __forceinline__ int operator()(int64_t i) const {
+    return keys ? keys[i] : key_of(index, is64, i, n_groups);
+  }
+};
+
+__global__ __launch_bounds__(kThreads) void count_kernel(Source src, int64_t n, int shift, int bits, int n_blocks,
+                                                         int32_t* __restrict__ hist) {
+  __shared__ int s_count[kMaxDigits];
+  const int digits = 1 << bits, mask = digits - 1;
+  for (int d = threadIdx.x; d < digits; d += kThreads) s_count[d] = 0;
+  __syncthreads();
+  const int64_t base = (int64_t)blockIdx.x * kTile;
+#pragma unroll
+  for (int r = 0; r < kTile / kThreads; ++r) {
+    const int64_t i = base + r * kThreads + threadIdx.x;
+    if (i < n) atomicAdd(&s_count[(src(i) >> shift) & mask], 1);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < digits; d += kThreads) hist[(int64_t)d * n_blocks + blockIdx.x] = s_count[d];
+}
+
+// one block per digit: hist[d][.] -> its exclusive prefix, totals[d]
+__global__ __launch_bounds__(kThreads) void scan_kernel(int32_t* __restrict__ hist, int n_blocks,
+                                                        int32_t* __restrict__ totals) {
+  __shared__ int s_wave[kThreads / 64];
+  int32_t* row = hist + (int64_t)blockIdx.x * n_blocks;
+  int run = 0;
+  for (int b = 0; b < n_blocks; b += kThreads) {
+    const int i = b + threadIdx.x;
+    const int v = i < n_blocks ? row[i] : 0;
+    int sum;
+    const int before = block_exclusive_scan<kThreads>(v, s_wave, &sum);
+    if (i < n_blocks) row[i] = run + before;
+    run += sum;
+  }
+  if (threadIdx.x == 0) totals[blockIdx.x] = run;
+}
+
+// offsets != nullptr (the sort's only pass): offsets[g] = start of digit g, g <= n_groups
+__global__ __launch_bounds__(kThreads) void scatter_kernel(Source src, const int32_t* __restrict__ order_in, int64_t n,
+                                                           int shift, int bits, int n_blocks,
+                                                           const int32_t* __restrict__ hist,
+                                                           const int32_t* __restrict__ totals,
+                                                           int32_t* __restrict__ keys_out,
+                                                           int32_t* __restrict__ order_out,
+                                                           int32_t* __restrict__ offsets, int n_groups) {
+  constexpr int kWaves = kThreads / 64, kPerWave = kTile / kWaves, kRounds = kPerWave / 64;
+  __shared__ int s_at[kWaves][kMaxDigits];
+  __shared__ int s_wave[kWaves];
+  const int digits = 1 << bits, mask = digits - 1;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int d = threadIdx.x; d < digits * kWaves; d += kThreads) s_at[d / digits][d % digits] = 0;
+  __syncthreads();
+  const int64_t base = (int64_t)blockIdx.x * kTile + wave * kPerWave + lane;
+  int key[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int64_t i = base + r * 64;
+    key[r] = i < n ? src(i) : -1;
+    if (i < n) atomicAdd(&s_at[wave][(key[r] >> shift) & mask], 1);
+  }
+  __syncthreads();
+  // s_at[w][d]: counts -> the place of wave w's first key with digit d
+  int start = 0;
+  for (int d0 = 0; d0 < digits; d0 += kThreads) {
+    const int d = d0 + threadIdx.x;
+    int sum;
+    const int before = block_exclusive_scan<kThreads>(d < digits ? totals[d] : 0, s_wave, &sum) + start;
+    start += sum;
+    if (d < digits) {
+      if (offsets && blockIdx.x == 0 && d <= n_groups) offsets[d] = before;
+      int at = before + hist[(int64_t)d * n_blocks + blockIdx.x];
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const int c = s_at[w][d];
+        s_at[w][d] = at;
+        at += c;
+      }
+    }
+  }
+  __syncthreads();
+  volatile int* my_at = s_at[wave];   // only this wave reads and writes it from here on
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int64_t i = base + r * 64;
+    const bool ok = i < n;
+    const int digit = (key[r] >> shift) & mask;
+    const uint64_t mine = same_digit(digit, bits, __ballot(ok));
+    const int below = __popcll(mine & ((1ull << lane) - 1));
+    int at = 0;
+    if (ok) at = my_at[digit] + below;
+    __builtin_amdgcn_wave_barrier();
+    if (ok && below == 0) my_at[digit] = at + __popcll(mine);
+    __builtin_amdgcn_wave_barrier();
+    if (ok) {
+      order_out[at] = order_in ? order_in[i] : (int32_t)i;
+      if (keys_out) keys_out[at] = key[r];
+    }
+  }
+}
+
+// first position of a sorted key >= v
+__device__ __forceinline__ int lower_bound(const int32_t* keys, int n, int v) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (keys[mid] < v) lo = mid + 1; else hi = mid;
+  }
+  return lo;
+}
+
+__global__ __launch_bounds__(kThreads) void offsets_kernel(const int32_t* __restrict__ keys, int64_t n, int n_groups,
+                                                           int32_t* __restrict__ offsets) {
+  const int64_t stride = (int64_t)gridDim.x * kThreads;
+  for (int64_t g = (int64_t)blockIdx.x * kThreads + threadIdx.x; g <= n_groups; g += stride)
+    offsets[g] = lower_bound(keys, (int)n, (int)g);
+}
+
+// All passes of at most kSmall keys in one workgroup; every wave owns a contiguous share of the positions.
+__global__ __launch_bounds__(kSmallThreads) void small_kernel(Source src, int n, int key_bits, int n_groups,
+                                                              int32_t* __restrict__ keys_out,
+                                                              int32_t* __restrict__ order_out,
+                                                              int32_t* __restrict__ offsets) {
+  constexpr int kWaves = kSmallThreads / 64, kDigits = 1 << kSmallBits;
+  __shared__ int s_key[2][kSmall];
+  __shared__ int s_row[2][kSmall];
+  __shared__ int s_at[kWaves][kDigits];
+  __shared__ int s_wave[kWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int rounds = (n + kSmallThreads - 1) / kSmallThreads;   // of 64 keys per wave
+  for (int i = tid; i < n; i += kSmallThreads) {
+    s_key[0][i] = src(i);
+    s_row[0][i] = i;
+  }
+  int cur = 0;
+  for (int shift = 0; shift < key_bits; shift += kSmallBits, cur ^= 1) {
+    const int bits = min(kSmallBits, key_bits - shift), mask = (1 << bits) - 1;
+    for (int d = tid; d < kWaves * kDigits; d += kSmallThreads) s_at[d / kDigits][d % kDigits] = 0;
+    __syncthreads();
+    for (int r = 0; r < rounds; ++r) {
+      const int i = (wave * rounds + r) * 64 + lane;
+      if (i < n) atomicAdd(&s_at[wave][(s_key[cur][i] >> shift) & mask], 1);
+    }
+    __syncthreads();
+    int count = 0;
+    if (tid < kDigits)
+      for (int w = 0; w < kWaves; ++w) count += s_at[w][tid];
+    int sum;
+    int at = block_exclusive_scan<kSmallThreads>(count, s_wave, &sum);
+    if (tid < kDigits)
+      for (int w = 0; w < kWaves; ++w) {
+        const int c = s_at[w][tid];
+        s_at[w][tid] = at;
+        at += c;
+      }
+    __syncthreads();
+    volatile int* my_at = s_at[wave];
+    for (int r = 0; r < rounds; ++r) {
+      const int i = (wave * rounds + r) * 64 + lane;
+      const bool ok = i < n;
+      const int key = ok ? s_key[cur][i] : 0;
+      const int digit = (key >> shift) & mask;
+      const uint64_t mine = same_digit(digit, bits, __ballot(ok));
+      const int below = __popcll(mine & ((1ull << lane) - 1));
+      int place = 0;
+      if (ok) place = my_at[digit] + below;
+      __builtin_amdgcn_wave_barrier();
+      if (ok && below == 0) my_at[digit] = place + __popcll(mine);
+      __builtin_amdgcn_wave_barrier();
+      if (ok) {
+        s_key[cur ^ 1][place] = key;
+        s_row[cur ^ 1][place] = s_row[cur][i];
+      }
+    }
+    __syncthreads();
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += kSmallThreads) {
+    order_out[i] = s_row[cur][i];
+    if (keys_out) keys_out[i] = s_key[cur][i];
+  }
+  if (offsets)
+    for (int g = tid; g <= n_groups; g += kSmallThreads) offsets[g] = lower_bound(s_key[cur], n, g);
+}
+
+// cumulative row counts (B,) -> offsets [B + 1], never decreasing and within 0 .. n whatever the counts hold
+__global__ __launch_bounds__(64) void offsets_from_counts_kernel(const void* cumulative, int is64, int n_groups,
+                                                                 int64_t n, int32_t* __restrict__ offsets) {
+  const int lane = threadIdx.x;
+  int run = 0;
+  if (lane == 0) offsets[0] = 0;
+  for (int g0 = 0; g0 < n_groups; g0 += 64) {
+    const int g = g0 + lane;
+    int64_t v = 0;
+    if (g < n_groups) v = is64 ? ((const int64_t*)cumulative)[g] : (int64_t)((const int32_t*)cumulative)[g];
+    int c = (int)(v < 0 ? 0 : v > n ? n : v);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int t = __shfl_up(c, d);
+      if (lane >= d) c = max(c, t);
+    }
+    c = max(c, run);
+    if (g < n_groups) offsets[g + 1] = c;
+    run = __shfl(c, 63);
+  }
+}
+
+int bits_for(int64_t n_groups) {   // keys 0 .. n_groups
+  int b = 1;
+  while (b < 31 && (1ll << b) <= n_groups) ++b;
+  return b;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t pv2_row_groups_workspace_ints(int64_t n, int64_t n_groups) {
+  if (n <= 0 || n_groups <= 0) return 1;
+  if (n <= kSmall) return n;
+  const int64_t n_blocks = (n + kTile - 1) / kTile;
+  return 3 * n + kMaxDigits * (n_blocks + 1);
+}
+
+int pv2_row_groups(const void* index, int index_is_64, int64_t n, int64_t n_groups, int32_t* order, int32_t* offsets,
+                   int32_t* sorted_ids, int32_t* workspace, pv2_stream_t stream) {
+  PV2_REQUIRE(offsets && n >= 0 && n < (1ll << 31) - kTile, "row_groups: bad row count");
+  PV2_REQUIRE(n_groups >= 1 && n_groups <= (1ll << 30), "row_groups: bad group count");
+  PV2_REQUIRE(n == 0 || (index && order && workspace), "row_groups: null pointer");
+  hipStream_t s = (hipStream_t)stream;
+  if (n == 0) return pv2::zero_words(offsets, n_groups + 1, s);
+  Source src{index, index_is_64, nullptr, (int)n_groups};
+  const int key_bits = bits_for(n_groups);
+  if (n <= kSmall) {
+    // (many offsets are searched by many blocks)
+    const bool inside = n_groups <= 8 * kSmallThreads;
+    int32_t* keys = sorted_ids ? sorted_ids : inside ? nullptr : workspace;
+    hipLaunchKernelGGL(small_kernel, dim3(1), dim3(kSmallThreads), 0, s, src, (int)n, key_bits, (int)n_groups, keys,
+                       order, inside ? offsets : nullptr);
+    if (!inside)
+      hipLaunchKernelGGL(offsets_kernel, dim3(pv2::grid_for(n_groups + 1, kThreads)), dim3(kThreads), 0, s, keys, n,
+                         (int)n_groups, offsets);
+    return pv2::check_launch("row_groups");
+  }
+  const int n_blocks = (int)((n + kTile - 1) / kTile);
+  const int passes = (key_bits + kMaxBits - 1) / kMaxBits;
+  const int bits = (key_bits + passes - 1) / passes;
+  int32_t* keys[2] = {workspace, workspace + n};
+  int32_t* other = workspace + 2 * n;
+  int32_t* hist = workspace + 3 * n;
+  int32_t* totals = hist + (int64_t)kMaxDigits * n_blocks;
+  const int32_t* order_in = nullptr;
+  for (int p = 0; p < passes; ++p) {
+    const bool last = p == passes - 1;
+    int32_t* order_out = ((passes - 1 - p) & 1) ? other : order;
+    int32_t* keys_out = last ? (sorted_ids ? sorted_ids : passes > 1 ? keys[p & 1] : nullptr) : keys[p & 1];
+    const int shift = p * bits, digits = 1 << bits;
+    hipLaunchKernelGGL(count_kernel, dim3(n_blocks), dim3(kThreads), 0, s, src, n, shift, bits, n_blocks, hist);
+    hipLaunchKernelGGL(scan_kernel, dim3(digits), dim3(kThreads), 0, s, hist, n_blocks, totals);
+    hipLaunchKernelGGL(scatter_kernel, dim3(n_blocks), dim3(kThreads), 0, s, src, order_in, n, shift, bits, n_blocks,
+                       hist, totals, keys_out, order_out, passes == 1 ? offsets : nullptr, (int)n_groups);
+    src.keys = keys_out;
+    order_in = order_out;
+  }
+  if (passes > 1)
+    hipLaunchKernelGGL(offsets_kernel, dim3(pv2::grid_for(n_groups + 1, kThreads)), dim3(kThreads), 0, s, src.keys, n,
+                       (int)n_groups, offsets);
+  return pv2::check_launch("row_groups");
+}
+
+int pv2_row_offsets(const void* cumulative, int is_64, int64_t n_groups, int64_t n, int32_t* offsets,
+                    pv2_stream_t stream) {
+  PV2_REQUIRE(cumulative && offsets, "row_offsets: null pointer");
+  PV2_REQUIRE(n >= 0 && n < (1ll << 31) - kTile && n_groups >= 1 && n_groups <= (1ll << 30), "row_offsets: bad shape");
+  hipLaunchKernelGGL(offsets_from_counts_kernel, dim3(1), dim3(64), 0, (hipStream_t)stream, cumulative, is_64,
+                     (int)n_groups, n, offsets);
+  return pv2::check_launch("row_offsets");
+}
+
+}  // extern "C"

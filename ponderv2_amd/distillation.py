@@ -1,0 +1,89 @@
+"""Distillation from a teacher's top logits: the classes and logits of a large (2-D, open-vocabulary) teacher are stored
+for its k best classes per row only (csrc/distillation.hip).
+
+With temperature T, p = softmax(teacher_logits / T) over a row's listed classes and q = softmax(logits / T) over all:
+``loss_i = T^2 * sum_e p_e (log p_e - log q_{c_e})``, the Kullback-Leibler divergence scaled so that its gradient keeps its
+size when T changes.  An entry counts if its class is one of the logits' (-1: none) and its logit is above -inf; a row
+without one has loss 0 and gradient 0, whatever its logits hold.  A class may be listed twice."""
+import math
+
+import torch
+
+from . import _lib
+from .kernels import DTYPE_CODE, _ptr, _require_device, _stream
+from .embedding import rows_contiguous
+from .row_groups import on_device, require_index
+
+MAX_TOP = 1024
+MAX_CLASSES = (1 << 30) - 1
+REDUCTIONS = ("mean", "sum", "none")
+
+
+class _TopkDistillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, index, teacher, temperature, reduction):
+        (m, v), k = logits.shape, index.shape[1]
+        L = _lib.lib()
+        new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=logits.device)
+        stats, loss, count = new(m, 2), new(), new()
+        row_loss = new(m) if reduction == "none" else None
+        workspace = new(int(L.pv2_topk_distill_workspace_floats(m, v, k)))
+        with on_device(logits):
+            _lib.check(L.pv2_topk_distill_forward(
+                _ptr(logits), DTYPE_CODE[logits.dtype], m, v, logits.stride(0), _ptr(index),
+                int(index.dtype == torch.int64), index.stride(0), _ptr(teacher), DTYPE_CODE[teacher.dtype],
+                teacher.stride(0), k, temperature, int(reduction == "mean"), _ptr(workspace), _ptr(stats),
+                _ptr(row_loss), _ptr(loss), _ptr(count), _stream(logits)), "pv2_topk_distill_forward")
+        ctx.save_for_backward(logits, index, teacher, stats, count)
+        ctx.how = (temperature, reduction)
+        return loss if row_loss is None else row_loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, up):
+        logits, index, teacher, stats, count = ctx.saved_tensors
+        temperature, reduction = ctx.how
+        (m, v), k = logits.shape, index.shape[1]
+        up = up.contiguous()
+        grad = torch.empty((m, v), dtype=logits.dtype, device=logits.device)
+        with on_device(logits):
+            _lib.check(_lib.lib().pv2_topk_distill_backward(
+                _ptr(logits), DTYPE_CODE[logits.dtype], m, v, logits.stride(0), _ptr(index),
+                int(index.dtype == torch.int64), index.stride(0), _ptr(teacher), DTYPE_CODE[teacher.dtype],
+                teacher.stride(0), k, temperature, _ptr(stats), _ptr(up), int(reduction == "none"),
+                _ptr(count) if reduction == "mean" else None, _ptr(grad), _stream(logits)),
+                "pv2_topk_distill_backward")
+        return grad, None, None, None, None
+
+
+def topk_distillation(logits, teacher_index, teacher_logits, temperature=1.0, reduction="mean"):
+    """logits (..., V) fp32 / bf16 / fp16; teacher_index (..., k) int64 / int32 and teacher_logits (..., k) fp32 / bf16 /
+    fp16, with the same leading axes.  -> fp32: the mean over the rows that count ("mean", 0 if none does), the sum, or
+    every row's loss ("none").  The gradient, of the logits only, has their type."""
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"topk_distillation: reduction is one of {REDUCTIONS}, got {reduction!r}")
+    temperature = float(temperature)
+    if not 0.0 < temperature < math.inf:
+        raise ValueError(f"topk_distillation: temperature is a positive number, got {temperature}")
+    require_index(teacher_index, "topk_distillation: teacher_index")
+    for name, t in (("logits", logits), ("teacher_logits", teacher_logits)):
+        if t.dtype not in DTYPE_CODE:
+            raise TypeError(f"topk_distillation: float32, bfloat16 or float16 {name} expected, got {t.dtype}")
+    if (logits.dim() < 1 or teacher_index.shape != teacher_logits.shape
+            or teacher_index.shape[:-1] != logits.shape[:-1] or teacher_index.dim() != logits.dim()):
+        raise ValueError(f"topk_distillation: logits (..., V), teacher_index and teacher_logits (..., k) expected, got "
+                         f"{tuple(logits.shape)}, {tuple(teacher_index.shape)}, {tuple(teacher_logits.shape)}")
+    v, k = logits.shape[-1], teacher_index.shape[-1]
+    if not 1 <= k <= MAX_TOP or not 1 <= v <= MAX_CLASSES:
+        raise ValueError(f"topk_distillation: {v} classes (1 to {MAX_CLASSES}), {k} listed (1 to {MAX_TOP})")
+    _require_device(logits, teacher_index, teacher_logits)
+    if not logits.device == teacher_index.device == teacher_logits.device:
+        raise ValueError("topk_distillation: logits, teacher_index and teacher_logits are on different devices")
+    lead = logits.shape[:-1]
+    if logits.numel() == 0:   # no rows: nothing to launch, an exact zero that still carries a gradient
+        empty = logits.float().sum(-1)
+        return empty if reduction == "none" else empty.sum()
+    loss = _TopkDistillation.apply(
+        rows_contiguous(logits.reshape(-1, v)), rows_contiguous(teacher_index.detach().reshape(-1, k)),
+        rows_contiguous(teacher_logits.detach().reshape(-1, k)), temperature, reduction)
+    return loss.reshape(lead) if reduction == "none" else loss

@@ -1,0 +1,64 @@
+"""Embedding lookup with scaling, its gradient by sorted tokens (csrc/embedding.hip).
+
+``embedding(index, weight, scale)`` is ``torch.nn.functional.embedding(index, weight) * scale`` for fp32 / bf16 / fp16
+tables, except that an index outside the table (-1: an unlabelled point, padding) gives a row of zeros and takes no
+gradient.  The gradient is dense, of the table's type, summed in fp32 in a fixed order: the same inputs give the same
+bits, however often a class repeats."""
+import torch
+
+from . import _lib
+from .kernels import DTYPE_CODE, _ptr, _require_device, _stream
+from .row_groups import MAX_GROUPS, MAX_ROWS, on_device, require_index
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, index, weight, scale):
+        n, (rows, c) = index.numel(), weight.shape
+        y = torch.empty((n, c), dtype=weight.dtype, device=weight.device)
+        if n:
+            with on_device(weight):
+                _lib.check(_lib.lib().pv2_embedding_forward(
+                    _ptr(index), int(index.dtype == torch.int64), n, _ptr(weight), DTYPE_CODE[weight.dtype], rows, c,
+                    weight.stride(0), scale, _ptr(y), _stream(weight)), "pv2_embedding_forward")
+        ctx.save_for_backward(index)
+        ctx.table = (rows, c, scale)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        index, = ctx.saved_tensors
+        rows, c, scale = ctx.table
+        n = index.numel()
+        gy = rows_contiguous(gy)
+        L = _lib.lib()
+        workspace = torch.empty(int(L.pv2_embedding_backward_workspace_ints(n, rows, c)), dtype=torch.int32,
+                                device=gy.device)
+        gw = torch.empty((rows, c), dtype=gy.dtype, device=gy.device)
+        with on_device(gy):
+            _lib.check(L.pv2_embedding_backward(
+                _ptr(index), int(index.dtype == torch.int64), n, _ptr(gy), DTYPE_CODE[gy.dtype], rows, c,
+                gy.stride(0), scale, _ptr(workspace), _ptr(gw), _stream(gy)), "pv2_embedding_backward")
+        return None, gw, None
+
+
+def rows_contiguous(t):
+    """A matrix whose rows are contiguous; any (non-negative) distance between rows is kept."""
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def embedding(index, weight, scale=1.0):
+    """index: int64 / int32 ids of any shape; weight (rows, C).  -> (*index.shape, C) = scale * weight[index]."""
+    require_index(index, "embedding")
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"embedding: weight is (rows, channels), got {tuple(weight.shape)}")
+    if weight.dtype not in DTYPE_CODE:
+        raise TypeError(f"embedding: float32, bfloat16 or float16 weight expected, got {weight.dtype}")
+    _require_device(index, weight)
+    if index.device != weight.device:
+        raise ValueError(f"embedding: index on {index.device}, weight on {weight.device}")
+    if index.numel() > MAX_ROWS or weight.shape[0] > MAX_GROUPS:
+        raise ValueError(f"embedding: up to {MAX_ROWS} indices and {MAX_GROUPS} rows")
+    y = _Embedding.apply(index.detach().reshape(-1), rows_contiguous(weight), float(scale))
+    return y.reshape(*index.shape, weight.shape[1])

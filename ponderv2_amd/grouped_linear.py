@@ -1,0 +1,95 @@
+"""Linear layers with weights of their own for each group of rows: experts, datasets, scenes (csrc/grouped_linear.hip).
+
+``grouped_linear(x, weight, groups, bias)`` is ``linear`` (linear.py) with ``weight[g]`` / ``bias[g]`` for the rows of
+group g: ``y[r] = x[r] @ weight[g].T + bias[g]``.  ``groups`` comes from ``row_groups.group_rows`` (rows in any order:
+they are read and written where they lie) or ``RowGroups.from_offset`` (rows that lie group by group).  Rows of no group
+are zeros in the result and take no gradient; groups may be empty (their weight gradient is zero).
+
+fp32, bf16 or fp16, one type for x, weight and bias, accumulated in fp32; the gradients (of x, weight and bias, once
+differentiable) are of the same type and summed in a fixed order.  fp32 products are formed from three bf16 pieces per
+operand: an infinity among them gives NaN where fp32 arithmetic would give an infinity."""
+import torch
+
+from . import _lib
+from .embedding import rows_contiguous
+from .kernels import DTYPE_CODE, _ptr, _require_device, _stream
+from .row_groups import RowGroups, on_device
+
+MAX_ROWS = (1 << 30) - 1
+MAX_GROUPS = (1 << 20) - 1
+MAX_WIDTH = (1 << 24) - 1
+
+
+class _GroupedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, order, offsets):
+        (m, k), (g, n, _) = x.shape, weight.shape
+        y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+        if m:
+            with on_device(x):
+                _lib.check(_lib.lib().pv2_grouped_linear_forward(
+                    _ptr(x), DTYPE_CODE[x.dtype], m, k, x.stride(0), _ptr(weight), weight.stride(0), weight.stride(1),
+                    g, n, _ptr(bias), _ptr(order), _ptr(offsets), _ptr(y), _stream(x)), "pv2_grouped_linear_forward")
+        ctx.save_for_backward(x, weight, order, offsets)
+        ctx.has_bias = bias is not None
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x, weight, order, offsets = ctx.saved_tensors
+        (m, k), (g, n, _) = x.shape, weight.shape
+        code, gy = DTYPE_CODE[x.dtype], rows_contiguous(gy)
+        L = _lib.lib()
+        new = lambda *shape, dtype=x.dtype: torch.empty(shape, dtype=dtype, device=x.device)
+        gx = gw = gb = None
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        if m == 0:
+            zeros = lambda *shape: torch.zeros(shape, dtype=x.dtype, device=x.device)
+            return (zeros(0, k) if need_x else None, zeros(g, n, k) if need_w else None,
+                    zeros(g, n) if need_b else None, None, None)
+        with on_device(x):
+            if need_x:
+                gx = new(m, k)
+                _lib.check(L.pv2_grouped_linear_grad_input(
+                    _ptr(gy), code, m, n, gy.stride(0), _ptr(weight), weight.stride(0), weight.stride(1), g, k,
+                    _ptr(order), _ptr(offsets), _ptr(gx), _stream(x)), "pv2_grouped_linear_grad_input")
+            if need_w or need_b:
+                gw = new(g, n, k)
+                gb = new(g, n) if need_b else None
+                floats = int(L.pv2_grouped_linear_workspace_floats(m, g, n, k))
+                workspace = new(floats, dtype=torch.float32) if floats else None
+                _lib.check(L.pv2_grouped_linear_grad_weight(
+                    _ptr(gy), code, m, n, gy.stride(0), _ptr(x), k, x.stride(0), g, _ptr(order), _ptr(offsets),
+                    _ptr(workspace), _ptr(gw), _ptr(gb), _stream(x)), "pv2_grouped_linear_grad_weight")
+        return gx, gw if need_w else None, gb, None, None
+
+
+def _weight_rows(w):
+    return w if w.stride(2) == 1 or w.shape[2] == 1 else w.contiguous()
+
+
+def grouped_linear(x, weight, groups, bias=None):
+    """x (M, K), weight (G, N, K), groups: RowGroups of M rows in G groups, bias (G, N) or None.  -> (M, N)."""
+    if not isinstance(groups, RowGroups):
+        raise TypeError("grouped_linear: groups is what row_groups.group_rows or RowGroups.from_offset returns")
+    if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2]:
+        raise ValueError(f"grouped_linear: x (M, K) and weight (G, N, K) expected, got {tuple(x.shape)} and "
+                         f"{tuple(weight.shape)}")
+    g, n, k = weight.shape
+    if groups.n_rows != x.shape[0] or groups.n_groups != g:
+        raise ValueError(f"grouped_linear: {x.shape[0]} rows and {g} weights, but groups of {groups.n_rows} rows in "
+                         f"{groups.n_groups} groups")
+    if bias is not None and tuple(bias.shape) != (g, n):
+        raise ValueError(f"grouped_linear: bias is (G, N) = {(g, n)}, got {tuple(bias.shape)}")
+    if min(n, k) < 1 or max(n, k) > MAX_WIDTH or x.shape[0] > MAX_ROWS or g > MAX_GROUPS:
+        raise ValueError(f"grouped_linear: widths 1 to {MAX_WIDTH}, up to {MAX_ROWS} rows and {MAX_GROUPS} groups")
+    tensors = [x, weight] + ([] if bias is None else [bias])
+    if x.dtype not in DTYPE_CODE or any(t.dtype != x.dtype for t in tensors):
+        raise TypeError("grouped_linear: x, weight and bias are all float32, all bfloat16 or all float16, got "
+                        + ", ".join(str(t.dtype) for t in tensors))
+    _require_device(*tensors)
+    if any(t.device != x.device for t in tensors + [groups.offsets]):
+        raise ValueError("grouped_linear: x, weight, bias and groups are on different devices")
+    return _GroupedLinear.apply(rows_contiguous(x), _weight_rows(weight),
+                                None if bias is None else bias.contiguous(), groups.order, groups.offsets)

@@ -1,0 +1,77 @@
+"""Rows by id: which rows belong to which group (expert, dataset, class, scene), as the grouped linear layers
+(grouped_linear.py) take it (csrc/row_groups.hip).
+
+``group_rows(index, num_groups)`` sorts the rows by their id on the device, without a host read;
+``RowGroups.from_offset(offset, n_rows)`` takes rows that already lie group by group, as the points of a batch do
+(``offset``: cumulative row counts, the ``data_dict["offset"]`` convention).
+"""
+import contextlib
+
+import torch
+
+from . import _lib
+from .kernels import _ptr, _require_device, _stream
+
+MAX_ROWS = (1 << 31) - 4097
+MAX_GROUPS = 1 << 30
+
+
+def on_device(t):
+    """Kernels are launched on ``t``'s device, whichever is current."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def require_index(index, what):
+    if index.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{what}: integer ids (int64 or int32) expected, got {index.dtype}")
+
+
+class RowGroups:
+    """``order`` int32 (n_rows,), or None where the rows already lie in order: the rows of group 0, of group 1, ..,
+    then the rows of no group; ``offsets`` int32 (n_groups + 1,): where each group's rows begin in it."""
+
+    __slots__ = ("order", "offsets", "n_rows", "n_groups")
+
+    def __init__(self, order, offsets, n_rows, n_groups):
+        self.order, self.offsets, self.n_rows, self.n_groups = order, offsets, n_rows, n_groups
+
+    @classmethod
+    def from_offset(cls, offset, n_rows):
+        """Rows 0 .. offset[0] - 1 are group 0's, offset[0] .. offset[1] - 1 group 1's, ..; rows behind the last
+        offset belong to no group."""
+        require_index(offset, "RowGroups.from_offset")
+        if offset.dim() != 1 or offset.numel() < 1:
+            raise ValueError("RowGroups.from_offset: offset is (n_groups,), one group at least")
+        if not 0 <= n_rows <= MAX_ROWS:
+            raise ValueError(f"RowGroups.from_offset: {n_rows} rows (0 to {MAX_ROWS})")
+        _require_device(offset)
+        offset = offset.detach().contiguous()
+        n_groups = offset.numel()
+        offsets = torch.empty(n_groups + 1, dtype=torch.int32, device=offset.device)
+        with on_device(offset):
+            _lib.check(_lib.lib().pv2_row_offsets(_ptr(offset), int(offset.dtype == torch.int64), n_groups, n_rows,
+                                                  _ptr(offsets), _stream(offset)), "pv2_row_offsets")
+        return cls(None, offsets, n_rows, n_groups)
+
+
+def group_rows(index, num_groups):
+    """index: integer ids of the rows (any shape, read as one list).  -> RowGroups with the stable order by id; rows
+    whose id is outside 0 .. num_groups - 1 (padding, unlabelled points at -1) belong to no group."""
+    require_index(index, "group_rows")
+    n = index.numel()
+    if not 1 <= num_groups <= MAX_GROUPS:
+        raise ValueError(f"group_rows: {num_groups} groups (1 to {MAX_GROUPS})")
+    if n > MAX_ROWS:
+        raise ValueError(f"group_rows: {n} rows (up to {MAX_ROWS})")
+    _require_device(index)
+    index = index.detach().contiguous()
+    L = _lib.lib()
+    ints = dict(dtype=torch.int32, device=index.device)
+    order, offsets = torch.empty(n, **ints), torch.empty(num_groups + 1, **ints)
+    workspace = torch.empty(int(L.pv2_row_groups_workspace_ints(n, num_groups)), **ints)
+    with on_device(index):
+        _lib.check(L.pv2_row_groups(_ptr(index), int(index.dtype == torch.int64), n, num_groups, _ptr(order),
+                                    _ptr(offsets), None, _ptr(workspace), _stream(index)), "pv2_row_groups")
+    return RowGroups(order, offsets, n, num_groups)
