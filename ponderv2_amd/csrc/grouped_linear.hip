@@ -13,6 +13,8 @@
 //                  partial results a second launch adds in order (no atomics).  db rides along as a product with ones.
 // few_rows_kernel  Y for a handful of rows (serving): bound by reading the weights once; 16 output columns per
 //                  workgroup, the reduction split over its four waves, operands straight from memory to registers.
+#include <type_traits>
+
 #include "common.h"
 #include "mfma_split.h"
 
@@ -37,6 +39,7 @@ struct __attribute__((packed, aligned(2))) Any8 { uint2 v; };
 template <typename H>
 struct Half {
   typedef u16 E;
+  typedef H Type;
   static constexpr int kPlanes = 1, kDepth = 64;   // depth: reduction steps staged at a time
   struct Raw { uint4 v; };                         // eight elements
   static __device__ __forceinline__ Raw zero() { return {make_uint4(0u, 0u, 0u, 0u)}; }
@@ -52,6 +55,12 @@ struct Half {
   static __device__ __forceinline__ u16x8 ones() { return (u16x8)(H::kOne); }
   static __device__ __forceinline__ float to_float(E v) { return H::to_float(v); }
   static __device__ __forceinline__ E from_float(float v) { return H::from_float(v); }
+  static __device__ __forceinline__ void put4(E* lds, const float* v) {
+    u16x4 t;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[j] = H::from_float(v[j]);
+    *reinterpret_cast<u16x4*>(lds) = t;
+  }
   static __device__ __forceinline__ void store4(E* p, const float* v, int count) {
     if (count >= 4) {
       u16x4 t;
@@ -117,6 +126,9 @@ struct Full {   // fp32: three bf16 planes in LDS
   static __device__ __forceinline__ u16x8 ones() { return (u16x8)(Bf::kOne); }
   static __device__ __forceinline__ float to_float(E v) { return v; }
   static __device__ __forceinline__ E from_float(float v) { return v; }
+  static __device__ __forceinline__ void put4(E* lds, const float* v) {
+    *reinterpret_cast<float4*>(lds) = make_float4(v[0], v[1], v[2], v[3]);
+  }
   static __device__ __forceinline__ void store4(E* p, const float* v, int count) {
     struct __attribute__((packed, aligned(4))) Any { float4 v; };
     if (count >= 4) {
@@ -133,14 +145,14 @@ struct Full {   // fp32: three bf16 planes in LDS
 // rows that one read instruction touches lie in different banks
 // "along": 128 rows, the reduction (kDepth) along the row
 template <int DEPTH>
-__device__ __forceinline__ int along_swizzle(int row) { return DEPTH == 64 ? (row & 7) : ((row >> 1) & 3); }
+__device__ __forceinline__ int along_swizzle(int row) { return DEPTH == 64 ? ((row >> 1) & 7) : ((row >> 2) & 3); }
 template <int DEPTH>
 __device__ __forceinline__ u16x8 along_fragment(const u16* tile, int row, int chunk) {
   return *reinterpret_cast<const u16x8*>(tile + row * DEPTH + ((chunk ^ along_swizzle<DEPTH>(row)) << 3));
 }
 // "across": kDepth rows of the reduction, 128 columns along the row; read through the transposing LDS read: lane t of a
 // 16-lane group points at row t / 4, columns 4 (t % 4) .. of a 4 x 16 block and receives column t of it
-__device__ __forceinline__ int across_swizzle(int row) { return (row & 7) << 1; }
+__device__ __forceinline__ int across_swizzle(int row) { return (row & 3) << 2; }
 __device__ __forceinline__ u16x8 across_fragment(const u16* tile, int step, int block, int lane) {
   typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
   const int g = lane >> 4, t = lane & 15;
@@ -166,28 +178,43 @@ struct Item {
   int base;        // the group's first item
 };
 
-// Item `item` when every group's rows are cut into pieces of `unit` (`empty`: a group without rows has one item, and
-// the rows of no group have none).  By a whole wave.
+// The item of workgroup `id` when every group's rows are cut into pieces of `unit` (`empty`: a group without rows has one
+// item, and the rows of no group have none), and its tile of `tiles`.  By a whole wave.  Workgroups are dealt to the 8
+// XCDs in turn; each XCD takes a contiguous eighth of the items, tile by tile, so that its L2 holds few groups' weights
+// and an item's rows are read into one L2 only (items dealt in turn instead: 124 -> 100 us for 32768 rows, 16 groups,
+// 1024 x 1024, bf16).
 __device__ __forceinline__ Item find_item(const int32_t* __restrict__ offsets, int n_groups, int n_rows, int unit,
-                                          bool empty, int item) {
+                                          bool empty, int id, int tiles, int* item_out, int* tile) {
   const int lane = threadIdx.x & 63;
-  Item it = {-1, 0, 0, 0, 0, 0};
-  int run = 0;
-  for (int g0 = 0; g0 <= n_groups; g0 += 64) {
+  int from = 0, to = 0, count = 0, upto = 0;
+  auto scan = [&](int g0) {   // counts of groups g0 .. g0 + 63 and their prefix sums
     const int g = g0 + lane;
-    int from = 0, to = 0;
+    from = to = 0;
     if (g <= n_groups) {
       from = offsets[g];
       to = g < n_groups ? offsets[g + 1] : n_rows;
     }
-    int count = (to - from + unit - 1) / unit;
+    count = (to - from + unit - 1) / unit;
     if (empty) count = g < n_groups ? max(count, 1) : 0;
-    int upto = count;
+    upto = count;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int t = __shfl_up(upto, d);
       if (lane >= d) upto += t;
     }
+    return __shfl(upto, 63);
+  };
+  int total = 0;
+  for (int g0 = 0; g0 <= n_groups; g0 += 64) total += scan(g0);
+  const int per_xcd = (total + 7) / 8, k = id / 8 / tiles;
+  const int item = id % 8 * per_xcd + k;
+  *tile = id / 8 % tiles;
+  *item_out = item;
+  Item it = {-1, 0, 0, 0, 0, 0};
+  if (k >= per_xcd || item >= total) return it;
+  int run = 0;
+  for (int g0 = 0; g0 <= n_groups; g0 += 64) {
+    const int sum = n_groups < 64 ? total : scan(g0);   // (one round: it is there already)
     const uint64_t past = __ballot(run + upto > item);
     if (past) {
       const int l = __ffsll((unsigned long long)past) - 1;
@@ -200,43 +227,70 @@ __device__ __forceinline__ Item find_item(const int32_t* __restrict__ offsets, i
       it.last = min(t, it.first + unit);
       return it;
     }
-    run += __shfl(upto, 63);
+    run += sum;
   }
   return it;
 }
 
-// Workgroups are dealt to the 8 XCDs in turn; an XCD takes whole items, tile by tile, so that an item's rows are read
-// into one L2 only.
-__device__ __forceinline__ void item_and_tile(int id, int tiles, int* item, int* tile) {
-  *item = id / (8 * tiles) * 8 + id % 8;
-  *tile = id / 8 % tiles;
+// An output tile leaves through LDS, so that rows are written in whole cache lines (an accumulator register holds one
+// element of 32 different rows).  `buffer`: 64 rows of kOutRow elements, this wave's 64 columns (tile columns 64 wc ..) of
+// its rows 32 b .. of each half: row 32 wr + i of the buffer is row 64 wr + 32 b + i of the tile.
+template <typename E, int COLS = kTile>
+constexpr int kOutRow = COLS + 16 / sizeof(E);
+// the buffer's ROWS rows of COLS elements -> dst(row)[0 .. count), by the whole workgroup; dst: nullptr for no such row
+template <int ROWS, int COLS, int THREADS = kThreads, typename E, typename Dst>
+__device__ __forceinline__ void write_rows(const E* buffer, int count, Dst dst) {
+  constexpr int N = 16 / sizeof(E), kPerRow = COLS / N;
+#pragma unroll 4
+  for (int q = threadIdx.x; q < ROWS * kPerRow; q += THREADS) {
+    const int row = q / kPerRow, col = q % kPerRow * N;
+    E* p = dst(row);
+    if (p == nullptr || col >= count) continue;
+    const E* src = buffer + row * kOutRow<E, COLS> + col;
+    if (col + N <= count) {
+      reinterpret_cast<Any16*>(p + col)->v = *reinterpret_cast<const uint4*>(src);
+    } else {
+      for (int j = 0; j < count - col; ++j) p[col + j] = src[j];
+    }
+  }
+}
+
+template <class P>
+__device__ __forceinline__ float load_bias(const typename P::E* __restrict__ bias, int group, int n_groups, int col,
+                                           int cols) {
+  return bias && group < n_groups && col < cols ? P::to_float(bias[(int64_t)group * cols + col]) : 0.f;
 }
 
 // A tile's chunks, held by the workgroup's threads between memory and LDS
 template <class P>
 constexpr int kChunks = kTile * P::kDepth / 8 / kThreads;
+// LDS of both operands' tiles or half an fp32 output tile, in 16-bit elements
+template <class P>
+constexpr int kLds = 2 * P::kPlanes * kTile * P::kDepth > 64 * kOutRow<float> * 2 ? 2 * P::kPlanes * kTile * P::kDepth
+                                                                                  : 64 * kOutRow<float> * 2;
 
 // WACROSS: the weights' reduction runs across their rows (dX: W is [reduction, columns]) instead of along them (Y)
 template <class P, bool WACROSS>
-__global__ __launch_bounds__(kThreads, P::kPlanes == 1 ? 2 : 2) void rows_kernel(
+__global__ __launch_bounds__(kThreads, 3) void rows_kernel(
     const typename P::E* __restrict__ x, int64_t ldx, const typename P::E* __restrict__ w, int64_t w_group,
     int64_t ldw, const typename P::E* __restrict__ bias, const int32_t* __restrict__ order,
     const int32_t* __restrict__ offsets, int n_rows, int n_groups, int cols, int depth, int n_tiles,
     typename P::E* __restrict__ y) {
   typedef typename P::E E;
   constexpr int D = P::kDepth, PL = P::kPlanes, kPlane = kTile * D, U = kChunks<P>;
-  __shared__ __attribute__((aligned(16))) u16 s_w[PL * kPlane];
-  __shared__ __attribute__((aligned(16))) u16 s_x[PL * kPlane];
+  __shared__ __attribute__((aligned(16))) u16 s_all[kLds<P>];
+  u16 *s_w = s_all, *s_x = s_all + PL * kPlane;
   __shared__ int s_row[kTile];
+  __shared__ __attribute__((aligned(16))) float s_bias[kTile];
   int item, tile;
-  item_and_tile(blockIdx.x, n_tiles, &item, &tile);
-  const Item it = find_item(offsets, n_groups, n_rows, kTile, false, item);
+  const Item it = find_item(offsets, n_groups, n_rows, kTile, false, blockIdx.x, n_tiles, &item, &tile);
   if (it.group < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int c0 = tile * kTile;
   if (tid < kTile) {
     const int p = it.first + tid;
     s_row[tid] = p < it.last ? (order ? order[p] : p) : -1;
+    s_bias[tid] = load_bias<P>(bias, it.group, n_groups, c0 + tid, cols);
   }
   __syncthreads();
   if (it.group == n_groups) {   // rows of no group: zeros
@@ -314,24 +368,25 @@ __global__ __launch_bounds__(kThreads, P::kPlanes == 1 ? 2 : 2) void rows_kernel
     }
   }
 
+  E* out = reinterpret_cast<E*>(s_all);
 #pragma unroll
   for (int b = 0; b < 2; ++b) {
-    const int r = s_row[wr * 64 + b * 32 + i];
-    if (r < 0) continue;
+    __syncthreads();   // the operands, or the first half of the tile, have been read
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int col = c0 + wc * 64 + a * 32 + 8 * q + 4 * h;
-        if (col >= cols) continue;
-        float v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[j] = acc[a][b][4 * q + j];
-          if (bias && col + j < cols) v[j] += P::to_float(bias[(int64_t)it.group * cols + col + j]);
-        }
-        P::store4(y + (int64_t)r * cols + col, v, cols - col);
+        const int col = wc * 64 + a * 32 + 8 * q + 4 * h;
+        const float4 add = *reinterpret_cast<const float4*>(s_bias + col);
+        const float v[4] = {acc[a][b][4 * q] + add.x, acc[a][b][4 * q + 1] + add.y, acc[a][b][4 * q + 2] + add.z,
+                            acc[a][b][4 * q + 3] + add.w};
+        P::put4(out + (wr * 32 + i) * kOutRow<E> + col, v);
       }
+    __syncthreads();
+    write_rows<64, kTile>(out, cols - c0, [&](int row) -> E* {
+      const int r = s_row[(row >> 5) * 64 + b * 32 + (row & 31)];
+      return r < 0 ? nullptr : y + (int64_t)r * cols + c0;
+    });
   }
 }
 
@@ -344,11 +399,10 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(
     float* __restrict__ dw_part, float* __restrict__ db_part) {
   typedef typename P::E E;
   constexpr int D = P::kDepth, PL = P::kPlanes, kPlane = kTile * D, U = kChunks<P>;
-  __shared__ __attribute__((aligned(16))) u16 s_x[PL * kPlane];
-  __shared__ __attribute__((aligned(16))) u16 s_g[PL * kPlane];
+  __shared__ __attribute__((aligned(16))) u16 s_all[kLds<P>];
+  u16 *s_x = s_all, *s_g = s_all + PL * kPlane;
   int item, tile;
-  item_and_tile(blockIdx.x, tiles_out * tiles_in, &item, &tile);
-  const Item it = find_item(offsets, n_groups, n_rows, unit, true, item);
+  const Item it = find_item(offsets, n_groups, n_rows, unit, true, blockIdx.x, tiles_out * tiles_in, &item, &tile);
   if (it.group < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int n0 = tile / tiles_in * kTile, k0 = tile % tiles_in * kTile;
@@ -427,26 +481,449 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(
   }
 
   const bool whole = it.of == 1;
+  auto leave = [&](auto* out, auto* base) {
+    typedef std::remove_pointer_t<decltype(out)> O;
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    const int n = n0 + wn * 64 + b * 32 + i;
-    if (n >= n_out) continue;
-    if (sum_bias && h == 0) {
+    for (int b = 0; b < 2; ++b) {
+      __syncthreads();
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = acc[a][b][4 * q + j];
+          O* at = out + (wn * 32 + i) * kOutRow<O> + wk * 64 + a * 32 + 8 * q + 4 * h;
+          if constexpr (sizeof(O) == 4) Full::put4(at, v);
+          else P::put4(at, v);
+        }
+      __syncthreads();
+      write_rows<64, kTile>(out, n_in - k0, [&](int row) -> O* {
+        const int n = n0 + (row >> 5) * 64 + b * 32 + (row & 31);
+        return n < n_out ? base + (int64_t)n * n_in + k0 : nullptr;
+      });
+    }
+  };
+  const int64_t size = (int64_t)n_out * n_in;
+  if (whole) leave(reinterpret_cast<E*>(s_all), dw + it.group * size);
+  else leave(reinterpret_cast<float*>(s_all), dw_part + item * size);
+  if (sum_bias && h == 0) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int n = n0 + wn * 64 + b * 32 + i;
+      if (n >= n_out) continue;
       if (whole) db[(int64_t)it.group * n_out + n] = P::from_float(acc_b[b][0]);
       else db_part[(int64_t)item * n_out + n] = acc_b[b][0];
     }
+  }
+}
+
+// ---- 16-bit operands whose rows are aligned to 16 bytes: memory -> LDS without registers in between.  Steps of 32 go
+// through three LDS buffers, two steps ahead of the products; a wave waits for its own loads of the next step (vmcnt
+// counts them) and for its reads of this one before the barrier that ends the step.  A chunk that is not there (a row
+// past the group, a column past the matrix, a step past the end) comes from a page of zeros, so that every step has the
+// same loads.
+constexpr int kStep = 32, kBuffers = 3;   // of the weight gradient
+__device__ uint4 g_zeros[4];   // never written
+
+template <int N>
+__device__ __forceinline__ void wait_for_loads() {   // all but the last N; and for all LDS reads
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));
+  asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+// 16 bytes per lane: the wave's 1 KB of LDS at `lds` (the same for all lanes), lane by lane
+__device__ __forceinline__ void load_to_lds(const u16* p, u16* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) unsigned*)p,
+                                   (__attribute__((address_space(3))) unsigned*)lds, 16, 0, 0);
+}
+
+// a lane's place in the chunks of an "along" / "across" tile of 32 reduction steps and its fragments
+constexpr int kDeep = 64;   // reduction steps of the row products' tiles
+__device__ __forceinline__ int along_row(int q) { return q / (kDeep / 8); }
+__device__ __forceinline__ int along_chunk(int q) { return (q % (kDeep / 8)) ^ along_swizzle<kDeep>(q / (kDeep / 8)); }
+template <int COLS>
+__device__ __forceinline__ int across_row(int q) { return q / (COLS / 8); }
+template <int COLS>
+__device__ __forceinline__ int across_chunk(int q) { return (q % (COLS / 8)) ^ across_swizzle(q / (COLS / 8)); }
+
+// Fragments are read in assembly: for its own LDS reads the compiler would wait for every load into LDS, those two steps
+// ahead as well.  Each block waits for its reads itself.
+typedef u16 u16x4v __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+__device__ __forceinline__ u16x8 glue(u16x4v lo, u16x4v hi) { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+// an "along" tile: N blocks of 32 rows, 4 KB apart
+template <int N>
+__device__ __forceinline__ void read_along(unsigned at, u16x8* f) {
+  static_assert(N == 2, "");
+  asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:4096\n\ts_waitcnt lgkmcnt(0)"
+               : "=&v"(f[0]), "=&v"(f[1])
+               : "v"(at)
+               : "memory");
+}
+// an "along" tile's two blocks together with N of another
+template <int N>
+__device__ __forceinline__ void read_along2(unsigned at, unsigned at2, u16x8* f, u16x8* f2) {
+  static_assert(N == 2 || N == 4, "");
+  if constexpr (N == 2)
+    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %2, %5\n\tds_read_b128 %1, %4 offset:4096\n\t"
+                 "ds_read_b128 %3, %5 offset:4096\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f2[0]), "=&v"(f2[1])
+                 : "v"(at), "v"(at2)
+                 : "memory");
+  else
+    asm volatile("ds_read_b128 %0, %6\n\tds_read_b128 %1, %6 offset:4096\n\tds_read_b128 %2, %7\n\t"
+                 "ds_read_b128 %3, %7 offset:4096\n\tds_read_b128 %4, %7 offset:8192\n\t"
+                 "ds_read_b128 %5, %7 offset:12288\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f2[0]), "=&v"(f2[1]), "=&v"(f2[2]), "=&v"(f2[3])
+                 : "v"(at), "v"(at2)
+                 : "memory");
+}
+// N blocks of 32 columns of an "across" tile with rows of ROW bytes: two transposing reads each, four rows apart
+template <int N, int OFF, int ROW>
+__device__ __forceinline__ void read_across(const unsigned* at, u16x8* f) {
+  u16x4v a[N], b[N];
+  if constexpr (N == 2)
+    asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %2, %4 offset:%7\n\t"
+                 "ds_read_b64_tr_b16 %1, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(a[0]), "=&v"(a[1]), "=&v"(b[0]), "=&v"(b[1])
+                 : "v"(at[0]), "v"(at[1]), "n"(OFF), "n"(OFF + 4 * ROW)
+                 : "memory");
+  else
+    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %4, %8 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %1, %9 offset:%12\n\tds_read_b64_tr_b16 %5, %9 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %2, %10 offset:%12\n\tds_read_b64_tr_b16 %6, %10 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %3, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(a[0]), "=&v"(a[1]), "=&v"(a[2]), "=&v"(a[3]), "=&v"(b[0]), "=&v"(b[1]), "=&v"(b[2]), "=&v"(b[3])
+                 : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(OFF), "n"(OFF + 4 * ROW)
+                 : "memory");
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+  for (int n = 0; n < N; ++n) f[n] = glue(a[n], b[n]);
+}
+// where a lane reads: block `block` of a tile (first step)
+__device__ __forceinline__ unsigned along_at(const u16* tile, int row, int chunk) {
+  return lds_address(tile + row * kDeep + ((chunk ^ along_swizzle<kDeep>(row)) << 3));
+}
+template <int COLS>
+__device__ __forceinline__ unsigned across_at(const u16* tile, int block, int lane) {
+  const int g = lane >> 4, t = lane & 15;
+  const int row = 8 * (g >> 1) + (t >> 2);   // (row + 4 and row + 16 have the same swizzle)
+  const int chunk = (block * 4 + 2 * (g & 1) + ((t & 3) >> 1)) ^ across_swizzle(row);
+  return lds_address(tile + row * COLS + (chunk << 3) + 4 * (t & 1));
+}
+
+// ROWS x COLS outputs per workgroup of ROWS / 32 waves, each with 64 rows and half of the columns
+template <class H, bool WACROSS, int ROWS, int COLS>
+__global__ __launch_bounds__(2 * ROWS, 2) void rows_direct_kernel(
+    const u16* __restrict__ x, int64_t ldx, const u16* __restrict__ w, int64_t w_group, int64_t ldw,
+    const u16* __restrict__ bias, const int32_t* __restrict__ order, const int32_t* __restrict__ offsets, int n_rows,
+    int n_groups, int cols, int depth, int n_tiles, u16* __restrict__ y) {
+  typedef Half<H> P;
+  constexpr int T = 2 * ROWS, A = COLS / 64, UX = ROWS * kDeep / 8 / T, UW = COLS * kDeep / 8 / T;
+  constexpr int kBuffer = (ROWS + COLS) * kDeep;
+  constexpr int kOut = ROWS * kOutRow<u16, COLS>;
+  __shared__ __attribute__((aligned(1024))) u16 s_all[2 * kBuffer > kOut ? 2 * kBuffer : kOut];   // (addresses are XORed)
+  __shared__ int s_row[ROWS];
+  __shared__ __attribute__((aligned(16))) float s_bias[COLS];
+  int item, tile;
+  const Item it = find_item(offsets, n_groups, n_rows, ROWS, false, blockIdx.x, n_tiles, &item, &tile);
+  if (it.group < 0) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c0 = tile * COLS;
+  if (tid < ROWS) {
+    const int p = it.first + tid;
+    s_row[tid] = p < it.last ? (order ? order[p] : p) : -1;
+  }
+  if (tid < COLS) s_bias[tid] = load_bias<P>(bias, it.group, n_groups, c0 + tid, cols);
+  __syncthreads();
+  if (it.group == n_groups) {   // rows of no group: zeros
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int q = tid; q < ROWS * COLS / 4; q += T) {
+      const int r = s_row[q / (COLS / 4)], col = c0 + q % (COLS / 4) * 4;
+      if (r >= 0 && col < cols) P::store4(y + (int64_t)r * cols + col, zero, cols - col);
+    }
+    return;
+  }
+  // This thread's chunks of a step.  A row past the group repeats the tile's first one and a column past the matrix the
+  // last one: what they give is not written.
+  const u16 *xp[UX], *wp[UW];
+#pragma unroll
+  for (int u = 0; u < UX; ++u) {
+    const int q = tid + u * T, r = s_row[along_row(q)];
+    xp[u] = x + (int64_t)(r >= 0 ? r : s_row[0]) * ldx + along_chunk(q) * 8;
+  }
+#pragma unroll
+  for (int u = 0; u < UW; ++u) {
+    const int q = tid + u * T;
+    const u16* wg = w + it.group * w_group;
+    wp[u] = WACROSS ? wg + across_row<COLS>(q) * ldw + min(c0 + across_chunk<COLS>(q) * 8, cols - 8)
+                    : wg + min(c0 + along_row(q), cols - 1) * ldw + along_chunk(q) * 8;
+  }
+  const int64_t w_add = WACROSS ? kDeep * ldw : kDeep;
+  int left = depth;   // reduction steps that are not loaded yet
+  // chunks FROM .. TO - 1 of the next step: x's, then the weights'
+  auto issue = [&](u16* to, auto from, auto until) {
+    to += wave * 64 * 8;
+    if (left >= kDeep) {
+#pragma unroll
+      for (int u = decltype(from)::value; u < decltype(until)::value; ++u) {
+        if (u < UX) {
+          load_to_lds(xp[u], to + u * T * 8);
+          xp[u] += kDeep;
+        } else {
+          load_to_lds(wp[u - UX], to + u * T * 8);
+          wp[u - UX] += w_add;
+        }
+      }
+    } else {   // the last, shorter step: zeros past the end
+      const u16* zeros = reinterpret_cast<const u16*>(g_zeros);
+#pragma unroll
+      for (int u = decltype(from)::value; u < decltype(until)::value; ++u) {
+        const int q = tid + (u < UX ? u : u - UX) * T;
+        const int k = u >= UX && WACROSS ? across_row<COLS>(q) : along_chunk(q) * 8;
+        load_to_lds(k < left ? (u < UX ? xp[u < UX ? u : 0] : wp[u < UX ? 0 : u - UX]) : zeros, to + u * T * 8);
+      }
+    }
+  };
+  static_assert(UX * T * 8 == ROWS * kDeep && UX + UW == 8, "");
+  using std::integral_constant;
+
+  f32x16 acc[A][2];
+#pragma unroll
+  for (int a = 0; a < A; ++a)
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) acc[a][b][q] = 0.f;
+  const int i = lane & 31, h = lane >> 5;
+  const int wc = wave & 1, wr = wave >> 1;
+  unsigned x_at = along_at(s_all, wr * 64 + i, h);
+  unsigned w_at = WACROSS ? across_at<COLS>(s_all + ROWS * kDeep, wc * A, lane)
+                          : along_at(s_all + ROWS * kDeep, wc * A * 32 + i, h);
+  int other = kBuffer;   // where the buffer that is not read now begins, from the one that is
+  u16* next = s_all;
+  issue(next, integral_constant<int, 0>(), integral_constant<int, 8>());
+  left -= kDeep;
+  wait_for_loads<0>();
+  barrier();
+  for (int k0 = 0; k0 < depth; k0 += kDeep) {
+    next += other;
+    auto quarter = [&](auto part) {
+      constexpr int s = decltype(part)::value;
+      // the loads of the next step go out in threes: a wave that issues all eight first starts its products late
+      constexpr int kFrom = s * 3 < 8 ? s * 3 : 8, kUntil = s * 3 + 3 < 8 ? s * 3 + 3 : 8;
+      if (left > 0) issue(next, integral_constant<int, kFrom>(), integral_constant<int, kUntil>());
+      u16x8 fw[A], fx[2];
+      if constexpr (WACROSS) {
+        unsigned at[A];
+#pragma unroll
+        for (int a = 0; a < A; ++a) at[a] = w_at ^ (a << 6);   // (block a: four chunks on)
+        read_along<2>(x_at ^ (s << 5), fx);
+        read_across<A, s * 16 * COLS * 2, COLS * 2>(at, fw);
+      } else {
+        read_along2<A>(x_at ^ (s << 5), w_at ^ (s << 5), fx, fw);
+      }
+#pragma unroll
+      for (int a = 0; a < A; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) acc[a][b] = H::mfma(fw[a], fx[b], acc[a][b]);
+    };
+    quarter(std::integral_constant<int, 0>());
+    quarter(std::integral_constant<int, 1>());
+    quarter(std::integral_constant<int, 2>());
+    quarter(std::integral_constant<int, 3>());
+    left -= kDeep;
+    x_at += other * 2;
+    w_at += other * 2;
+    other = -other;
+    wait_for_loads<0>();
+    barrier();
+  }
+
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+#pragma unroll
+    for (int a = 0; a < A; ++a)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int k = k0 + wk * 64 + a * 32 + 8 * q + 4 * h;
-        if (k >= n_in) continue;
-        float v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = acc[a][b][4 * q + j];
-        if (whole) P::store4(dw + ((int64_t)it.group * n_out + n) * n_in + k, v, n_in - k);
-        else Full::store4(dw_part + ((int64_t)item * n_out + n) * n_in + k, v, n_in - k);
+        const int col = (wc * A + a) * 32 + 8 * q + 4 * h;
+        const float4 add = *reinterpret_cast<const float4*>(s_bias + col);
+        const float v[4] = {acc[a][b][4 * q] + add.x, acc[a][b][4 * q + 1] + add.y, acc[a][b][4 * q + 2] + add.z,
+                            acc[a][b][4 * q + 3] + add.w};
+        P::put4(s_all + (wr * 64 + b * 32 + i) * kOutRow<u16, COLS> + col, v);
       }
+  __syncthreads();
+  write_rows<ROWS, COLS, T>(s_all, cols - c0, [&](int row) -> u16* {
+    const int r = s_row[row];
+    return r < 0 ? nullptr : y + (int64_t)r * cols + c0;
+  });
+}
+
+// dW of one item as wgrad_kernel: 128 rows n x COLS columns k; the item's row numbers pass through LDS, kSegment at a time
+constexpr int kSegment = 60 * kStep;
+template <class H, int COLS>
+__global__ __launch_bounds__(kThreads, 2) void wgrad_direct_kernel(
+    const u16* __restrict__ dy, int64_t ldy, const u16* __restrict__ x, int64_t ldx, const int32_t* __restrict__ order,
+    const int32_t* __restrict__ offsets, int n_rows, int n_groups, int n_out, int n_in, int unit, int tiles_out,
+    int tiles_in, u16* __restrict__ dw, u16* __restrict__ db, float* __restrict__ dw_part,
+    float* __restrict__ db_part) {
+  typedef Half<H> P;
+  constexpr int A = COLS / 64, UG = kTile * kStep / 8 / kThreads, UX = COLS * kStep / 8 / kThreads;
+  constexpr int kBuffer = (kTile + COLS) * kStep;
+  constexpr int kOut = 64 * kOutRow<float, COLS> * 2;
+  __shared__ __attribute__((aligned(16))) u16 s_all[kBuffers * kBuffer > kOut ? kBuffers * kBuffer : kOut];
+  __shared__ int s_row[kSegment];
+  int item, tile;
+  const Item it = find_item(offsets, n_groups, n_rows, unit, true, blockIdx.x, tiles_out * tiles_in, &item, &tile);
+  if (it.group < 0) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n0 = tile / tiles_in * kTile, k0 = tile % tiles_in * COLS;
+  const int i = lane & 31, h = lane >> 5;
+  const int wk = wave & 1, wn = wave >> 1;
+  const bool sum_bias = db != nullptr && k0 == 0 && wk == 0;
+  const u16* zeros = reinterpret_cast<const u16*>(g_zeros);
+
+  const int gcol = n0 + across_chunk<kTile>(tid) * 8, xcol = k0 + across_chunk<COLS>(tid) * 8;
+  static_assert(kThreads / (kTile / 8) % 4 == 0 && kThreads / (COLS / 8) % 4 == 0, "the same swizzle for all chunks");
+  int segment_rows = 0, at = 0;   // rows of this segment and position of the next step in it
+  // the row numbers of the next step's chunks, read a step ahead (positions past the segment: any, not used)
+  int g_row[UG], x_row[UX];
+  auto next_rows = [&]() {
+    const int last = kSegment - kStep;
+    const unsigned from = lds_address(s_row + min(at, last));
+    const unsigned ga = from + across_row<kTile>(tid) * 4, xa = from + across_row<COLS>(tid) * 4;
+    constexpr int G = kThreads / (kTile / 8) * 4, X = kThreads / (COLS / 8) * 4;
+    if constexpr (UX == 4)
+      asm volatile("ds_read_b32 %0, %6\n\tds_read_b32 %1, %6 offset:%8\n\tds_read_b32 %2, %7\n\tds_read_b32 %3, %7 offset:%9\n\t"
+                   "ds_read_b32 %4, %7 offset:%10\n\tds_read_b32 %5, %7 offset:%11\n\ts_waitcnt lgkmcnt(0)"
+                   : "=&v"(g_row[0]), "=&v"(g_row[1]), "=&v"(x_row[0]), "=&v"(x_row[1]), "=&v"(x_row[2]), "=&v"(x_row[3])
+                   : "v"(ga), "v"(xa), "n"(G), "n"(X), "n"(2 * X), "n"(3 * X)
+                   : "memory");
+    else
+      asm volatile("ds_read_b32 %0, %4\n\tds_read_b32 %1, %4 offset:%6\n\tds_read_b32 %2, %5\n\tds_read_b32 %3, %5 offset:%7\n\t"
+                   "s_waitcnt lgkmcnt(0)"
+                   : "=&v"(g_row[0]), "=&v"(g_row[1]), "=&v"(x_row[0]), "=&v"(x_row[1])
+                   : "v"(ga), "v"(xa), "n"(G), "n"(X)
+                   : "memory");
+  };
+  auto issue = [&](int buffer) {
+    u16* to = s_all + buffer * kBuffer + wave * 64 * 8;
+#pragma unroll
+    for (int u = 0; u < UG; ++u) {
+      const bool ok = at + across_row<kTile>(tid + u * kThreads) < segment_rows && gcol < n_out;
+      load_to_lds(ok ? dy + (int64_t)g_row[u] * ldy + gcol : zeros, to + u * kThreads * 8);
+    }
+#pragma unroll
+    for (int u = 0; u < UX; ++u) {
+      const bool ok = at + across_row<COLS>(tid + u * kThreads) < segment_rows && xcol < n_in;
+      load_to_lds(ok ? x + (int64_t)x_row[u] * ldx + xcol : zeros, to + kTile * kStep + u * kThreads * 8);
+    }
+    at += kStep;
+    next_rows();
+  };
+
+  f32x16 acc[A][2], acc_b[2];
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+      acc_b[b][q] = 0.f;
+#pragma unroll
+      for (int a = 0; a < A; ++a) acc[a][b][q] = 0.f;
+    }
+  unsigned g_at[2], x_at[A];
+#pragma unroll
+  for (int b = 0; b < 2; ++b) g_at[b] = across_at<kTile>(s_all, wn * 2 + b, lane);
+#pragma unroll
+  for (int a = 0; a < A; ++a) x_at[a] = across_at<COLS>(s_all + kTile * kStep, wk * A + a, lane);
+  auto step = [&](auto buffer, int next) {
+    constexpr int kAt = decltype(buffer)::value * kBuffer * 2;
+    u16x8 fx[A], fg[2];
+    auto products = [&]() {
+#pragma unroll
+      for (int a = 0; a < A; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) acc[a][b] = H::mfma(fx[a], fg[b], acc[a][b]);
+      if (sum_bias) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) acc_b[b] = H::mfma(P::ones(), fg[b], acc_b[b]);
+      }
+    };
+    issue(next);
+    read_across<2, kAt, kTile * 2>(g_at, fg);
+    read_across<A, kAt, COLS * 2>(x_at, fx);
+    products();
+    read_across<2, kAt + 16 * kTile * 2, kTile * 2>(g_at, fg);
+    read_across<A, kAt + 16 * COLS * 2, COLS * 2>(x_at, fx);
+    products();
+    wait_for_loads<UG + UX>();
+    barrier();
+  };
+  for (int first = it.first; first < it.last; first += kSegment) {
+    segment_rows = min(kSegment, it.last - first);
+    at = 0;
+    for (int p = tid; p < segment_rows; p += kThreads) s_row[p] = order ? order[first + p] : first + p;
+    __syncthreads();
+    next_rows();
+    issue(0);
+    issue(1);
+    wait_for_loads<UG + UX>();
+    barrier();
+    for (int done = 0;; ) {
+      step(std::integral_constant<int, 0>(), 2);
+      if ((done += kStep) >= segment_rows) break;
+      step(std::integral_constant<int, 1>(), 0);
+      if ((done += kStep) >= segment_rows) break;
+      step(std::integral_constant<int, 2>(), 1);
+      if ((done += kStep) >= segment_rows) break;
+    }
+    wait_for_loads<0>();
+    barrier();
+  }
+
+  const bool whole = it.of == 1;
+  auto leave = [&](auto* out, auto* base) {
+    typedef std::remove_pointer_t<decltype(out)> O;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      __syncthreads();
+#pragma unroll
+      for (int a = 0; a < A; ++a)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = acc[a][b][4 * q + j];
+          O* to = out + (wn * 32 + i) * kOutRow<O, COLS> + (wk * A + a) * 32 + 8 * q + 4 * h;
+          if constexpr (sizeof(O) == 4) Full::put4(to, v);
+          else P::put4(to, v);
+        }
+      __syncthreads();
+      write_rows<64, COLS>(out, n_in - k0, [&](int row) -> O* {
+        const int n = n0 + (row >> 5) * 64 + b * 32 + (row & 31);
+        return n < n_out ? base + (int64_t)n * n_in + k0 : nullptr;
+      });
+    }
+  };
+  const int64_t size = (int64_t)n_out * n_in;
+  if (whole) leave(s_all, dw + it.group * size);
+  else leave(reinterpret_cast<float*>(s_all), dw_part + item * size);
+  if (sum_bias && h == 0) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int n = n0 + wn * 64 + b * 32 + i;
+      if (n >= n_out) continue;
+      if (whole) db[(int64_t)it.group * n_out + n] = H::from_float(acc_b[b][0]);
+      else db_part[(int64_t)item * n_out + n] = acc_b[b][0];
+    }
   }
 }
 
@@ -529,8 +1006,8 @@ __global__ __launch_bounds__(kThreads) void few_rows_kernel(
   typedef Few<P> F;
   constexpr int U = 4;
   __shared__ f32x4 s_part[kThreads / 64][64];
-  const int item = blockIdx.x / n_tiles, tile = blockIdx.x % n_tiles;
-  const Item it = find_item(offsets, n_groups, n_rows, 16, false, item);
+  int item, tile;
+  const Item it = find_item(offsets, n_groups, n_rows, 16, false, blockIdx.x, n_tiles, &item, &tile);
   if (it.group < 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i = lane & 15, h = lane >> 4;
@@ -589,6 +1066,19 @@ constexpr int64_t kMostBlocks = 1 << 24;   // of 256 threads
 // Serving: few rows to a group on average, so that the weights are what is read.
 bool few_rows(int64_t rows, int64_t groups) { return rows <= 16 || rows <= 4 * groups; }
 
+bool aligned16(const void* p, int64_t a, int64_t b, int elem) {
+  return (uintptr_t)p % 16 == 0 && a * elem % 16 == 0 && b * elem % 16 == 0;
+}
+
+// Columns of a weight gradient's 16-bit tile: 256 where that pads no more than 128 would.
+int wgrad_cols(int n_in) { return tiles_of(n_in, 128) % 2 ? 128 : 256; }
+
+// Tiles of 256 x 256 (bf16, 32768 rows, 16 groups, 1024 x 1024: 75 us against 90 with 128 x 128) where they fill the 256
+// CUs and pad no columns; else 128 x 128 (8192 rows: 26 us against 34).
+bool large_tiles(int64_t rows, int cols) {
+  return tiles_of(cols, 128) % 2 == 0 && rows / 256 * tiles_of(cols, 256) >= 256;
+}
+
 template <class P, bool WACROSS>
 int launch_rows(const void* x, int64_t ldx, const void* w, int64_t w_group, int64_t ldw, const void* bias,
                 const int32_t* order, const int32_t* offsets, int64_t rows, int64_t groups, int cols, int depth,
@@ -596,16 +1086,31 @@ int launch_rows(const void* x, int64_t ldx, const void* w, int64_t w_group, int6
   typedef typename P::E E;
   if (!WACROSS && few_rows(rows, groups)) {
     const int tiles = tiles_of(cols, 16);
-    const int64_t blocks = most_items(rows, groups, 16) * tiles;
+    const int64_t blocks = (most_items(rows, groups, 16) + 7) / 8 * 8 * tiles;
     PV2_REQUIRE(blocks < kMostBlocks, "grouped_linear: too many tiles");
     hipLaunchKernelGGL((few_rows_kernel<P>), dim3((unsigned)blocks), dim3(kThreads), 0, s, (const E*)x, ldx,
                        (const E*)w, w_group, ldw, (const E*)bias, order, offsets, (int)rows, (int)groups, cols, depth,
                        tiles, (E*)y);
     return pv2::check_launch("grouped_linear");
   }
-  const int tiles = tiles_of(cols, kTile);
-  const int64_t blocks = (most_items(rows, groups, kTile) + 7) / 8 * 8 * tiles;
+  const bool direct = sizeof(E) == 2 && aligned16(x, ldx, depth, 2) && aligned16(w, ldw, w_group, 2) &&
+                      (!WACROSS || cols % 8 == 0);
+  const int size = direct && large_tiles(rows, cols) ? 256 : 128;
+  const int tiles = tiles_of(cols, size);
+  const int64_t blocks = (most_items(rows, groups, size) + 7) / 8 * 8 * tiles;
   PV2_REQUIRE(blocks < kMostBlocks, "grouped_linear: too many tiles");
+  if constexpr (sizeof(E) == 2) {
+    if (direct) {
+#define PV2_DIRECT(ROWS, COLS)                                                                                       \
+  hipLaunchKernelGGL((rows_direct_kernel<typename P::Type, WACROSS, ROWS, COLS>), dim3((unsigned)blocks),            \
+                     dim3(2 * ROWS), 0, s, (const E*)x, ldx, (const E*)w, w_group, ldw, (const E*)bias, order, offsets, \
+                     (int)rows, (int)groups, cols, depth, tiles, (E*)y)
+      if (size == 256) PV2_DIRECT(256, 256);
+      else PV2_DIRECT(128, 128);
+#undef PV2_DIRECT
+      return pv2::check_launch("grouped_linear");
+    }
+  }
   hipLaunchKernelGGL((rows_kernel<P, WACROSS>), dim3((unsigned)blocks), dim3(kThreads), 0, s, (const E*)x, ldx,
                      (const E*)w, w_group, ldw, (const E*)bias, order, offsets, (int)rows, (int)groups, cols, depth,
                      tiles, (E*)y);
@@ -618,8 +1123,8 @@ struct Split {   // of the weight gradient
 };
 
 // About 512 workgroups where the rows allow it: two to a CU.
-Split split_of(int64_t rows, int64_t groups, int n_out, int n_in) {
-  const int64_t tiles = (int64_t)tiles_of(n_out, kTile) * tiles_of(n_in, kTile);
+Split split_of(int dtype, int64_t rows, int64_t groups, int n_out, int n_in) {
+  const int64_t tiles = (int64_t)tiles_of(n_out, kTile) * tiles_of(n_in, dtype == PV2_F32 ? kTile : wgrad_cols(n_in));
   const int64_t want = (512 + tiles - 1) / tiles;
   int64_t unit = (rows + want - 1) / want;
   if (unit < 256) unit = 256;
@@ -632,17 +1137,27 @@ int launch_wgrad(const void* dy, int64_t ldy, const void* x, int64_t ldx, const 
                  const int32_t* offsets, int64_t rows, int64_t groups, int n_out, int n_in, float* ws, void* dw,
                  void* db, hipStream_t s) {
   typedef typename P::E E;
-  const Split sp = split_of(rows, groups, n_out, n_in);
-  const int to = tiles_of(n_out, kTile), ti = tiles_of(n_in, kTile);
+  const Split sp = split_of(sizeof(E) == 4 ? PV2_F32 : PV2_BF16, rows, groups, n_out, n_in);
+  const bool direct = sizeof(E) == 2 && aligned16(dy, ldy, n_out, 2) && aligned16(x, ldx, n_in, 2);
+  const int tile_cols = direct ? wgrad_cols(n_in) : kTile;
+  const int to = tiles_of(n_out, kTile), ti = tiles_of(n_in, tile_cols);
   const int64_t blocks = (sp.items + 7) / 8 * 8 * to * ti;
   PV2_REQUIRE(blocks < kMostBlocks, "grouped_linear: too many tiles");
   const int64_t size = (int64_t)n_out * n_in;
   const bool parts = rows > sp.unit;
   PV2_REQUIRE(!parts || ws, "grouped_linear: no workspace");
   float* db_part = parts ? ws + sp.items * size : nullptr;
-  hipLaunchKernelGGL((wgrad_kernel<P>), dim3((unsigned)blocks), dim3(kThreads), 0, s, (const E*)dy, ldy, (const E*)x,
-                     ldx, order, offsets, (int)rows, (int)groups, n_out, n_in, sp.unit, to, ti, (E*)dw, (E*)db, ws,
-                     db_part);
+#define PV2_WGRAD(kernel)                                                                                            \
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), 0, s, (const E*)dy, ldy, (const E*)x, ldx, order, \
+                     offsets, (int)rows, (int)groups, n_out, n_in, sp.unit, to, ti, (E*)dw, (E*)db, ws, db_part)
+  if constexpr (sizeof(E) == 2) {
+    if (!direct) PV2_WGRAD((wgrad_kernel<P>));
+    else if (tile_cols == 256) PV2_WGRAD((wgrad_direct_kernel<typename P::Type, 256>));
+    else PV2_WGRAD((wgrad_direct_kernel<typename P::Type, 128>));
+  } else {
+    PV2_WGRAD((wgrad_kernel<P>));
+  }
+#undef PV2_WGRAD
   if (parts) {
     int64_t chunks = (size + kThreads - 1) / kThreads;
     const int64_t most = 1 + 4096 / groups;
@@ -697,9 +1212,9 @@ int pv2_grouped_linear_grad_input(const void* grad_out, int dtype, int64_t rows,
 #undef PV2_CALL
 }
 
-int64_t pv2_grouped_linear_workspace_floats(int64_t rows, int64_t groups, int n_out, int n_in) {
+int64_t pv2_grouped_linear_workspace_floats(int dtype, int64_t rows, int64_t groups, int n_out, int n_in) {
   if (rows < 1 || groups < 1 || n_out < 1 || n_in < 1) return 0;
-  const Split sp = split_of(rows, groups, n_out, n_in);
+  const Split sp = split_of(dtype, rows, groups, n_out, n_in);
   return rows > sp.unit ? sp.items * ((int64_t)n_out * n_in + n_out) : 0;
 }
 

@@ -57,7 +57,7 @@ class _GroupedLinear(torch.autograd.Function):
             if need_w or need_b:
                 gw = new(g, n, k)
                 gb = new(g, n) if need_b else None
-                floats = int(L.pv2_grouped_linear_workspace_floats(m, g, n, k))
+                floats = int(L.pv2_grouped_linear_workspace_floats(code, m, g, n, k))
                 workspace = new(floats, dtype=torch.float32) if floats else None
                 _lib.check(L.pv2_grouped_linear_grad_weight(
                     _ptr(gy), code, m, n, gy.stride(0), _ptr(x), k, x.stride(0), g, _ptr(order), _ptr(offsets),

@@ -135,7 +135,7 @@ def test_workspaces_cover_what_is_asked():
     L = _lib.lib()
     assert L.pv2_row_groups_workspace_ints(0, 5) >= 1
     assert L.pv2_row_groups_workspace_ints(100000, 5) >= 3 * 100000
-    assert L.pv2_grouped_linear_workspace_floats(100, 4, 64, 64) == 0          # no group can be split
+    assert L.pv2_grouped_linear_workspace_floats(0, 100, 4, 64, 64) == 0          # no group can be split
     # 3 groups of 512 x 96: four 128 x 128 tiles, at most 128 + 3 items
-    assert 0 < L.pv2_grouped_linear_workspace_floats(92417, 3, 512, 96) <= (128 + 3) * (512 * 96 + 512)
+    assert 0 < L.pv2_grouped_linear_workspace_floats(0, 92417, 3, 512, 96) <= (128 + 3) * (512 * 96 + 512)
     assert L.pv2_topk_distill_workspace_floats(1, 131072, 16) > 2
