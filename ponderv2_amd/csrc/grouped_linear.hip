@@ -10,7 +10,7 @@
 //
 // rows_kernel      Y and dX: a 128-row x 128-column tile per workgroup, four waves of 64 x 64.
 // wgrad_kernel     dW and db: a 128 x 128 tile of one group's dW; long groups are split over rows into items whose fp32
-//                  partial results a second launch adds in order (no atomics).  db rides along as a product with ones.
+//                  partial results a second launch adds in order (no atomics).  db is summed from the fragments of dY.
 // few_rows_kernel  Y for a handful of rows (serving): bound by reading the weights once; 16 output columns per
 //                  workgroup, the reduction split over its four waves, operands straight from memory to registers.
 #include <type_traits>
@@ -52,7 +52,12 @@ struct Half {
   }
   static __device__ __forceinline__ void stage(u16* lds, int, const Raw& r) { *reinterpret_cast<uint4*>(lds) = r.v; }
   static __device__ __forceinline__ f32x16 mfma(const u16x8* a, const u16x8* b, f32x16 c) { return H::mfma(a[0], b[0], c); }
-  static __device__ __forceinline__ u16x8 ones() { return (u16x8)(H::kOne); }
+  static __device__ __forceinline__ float sum(const u16x8& f) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += H::to_float(f[j]);
+    return s;
+  }
   static __device__ __forceinline__ float to_float(E v) { return H::to_float(v); }
   static __device__ __forceinline__ E from_float(float v) { return H::from_float(v); }
   static __device__ __forceinline__ void put4(E* lds, const float* v) {
@@ -76,7 +81,6 @@ struct Half {
 };
 
 struct Bf {
-  static constexpr u16 kOne = 0x3f80;
   static __device__ __forceinline__ f32x16 mfma(u16x8 a, u16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
@@ -88,7 +92,6 @@ struct Bf {
 };
 
 struct Hf {
-  static constexpr u16 kOne = 0x3c00;
   static __device__ __forceinline__ f32x16 mfma(u16x8 a, u16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
@@ -123,7 +126,7 @@ struct Full {   // fp32: three bf16 planes in LDS
 #undef PV2_TERM
     return c;
   }
-  static __device__ __forceinline__ u16x8 ones() { return (u16x8)(Bf::kOne); }
+  static __device__ __forceinline__ float sum(const u16x8& f) { return Half<Bf>::sum(f); }
   static __device__ __forceinline__ float to_float(E v) { return v; }
   static __device__ __forceinline__ E from_float(float v) { return v; }
   static __device__ __forceinline__ void put4(E* lds, const float* v) {
@@ -223,8 +226,10 @@ __device__ __forceinline__ Item find_item(const int32_t* __restrict__ offsets, i
       it.number = item - it.base;
       it.group = g0 + l;
       const int f = __shfl(from, l), t = __shfl(to, l);
-      it.first = f + it.number * unit;
-      it.last = min(t, it.first + unit);
+      // (a group's items of a weight gradient are about equal: whole steps of 32 rows, the last one may be empty)
+      const int piece = empty ? ((t - f + it.of - 1) / it.of + 31) / 32 * 32 : unit;
+      it.first = f + it.number * piece;
+      it.last = min(t, it.first + piece);
       return it;
     }
     run += sum;
@@ -392,7 +397,7 @@ __global__ __launch_bounds__(kThreads, 3) void rows_kernel(
 
 // dW[g][n][k] over one item's rows.  The item is the whole group: written in the weights' type; else fp32 partials.
 template <class P>
-__global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(
+__global__ __launch_bounds__(kThreads, 3) void wgrad_kernel(
     const typename P::E* __restrict__ dy, int64_t ldy, const typename P::E* __restrict__ x, int64_t ldx,
     const int32_t* __restrict__ order, const int32_t* __restrict__ offsets, int n_rows, int n_groups, int n_out,
     int n_in, int unit, int tiles_out, int tiles_in, typename P::E* __restrict__ dw, typename P::E* __restrict__ db,
@@ -430,11 +435,12 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(
     }
   };
 
-  f32x16 acc[2][2], acc_b[2];
+  f32x16 acc[2][2];
+  float bias_sum[2] = {0.f, 0.f};   // of this lane's column and its reduction steps
 #pragma unroll
   for (int b = 0; b < 2; ++b)
 #pragma unroll
-    for (int q = 0; q < 16; ++q) acc[0][b][q] = acc[1][b][q] = acc_b[b][q] = 0.f;
+    for (int q = 0; q < 16; ++q) acc[0][b][q] = acc[1][b][q] = 0.f;
 
   load_rows(it.first);
   load();
@@ -467,15 +473,10 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(
 #pragma unroll
         for (int b = 0; b < 2; ++b) acc[a][b] = P::mfma(fx[a], fg[b], acc[a][b]);
       if (sum_bias) {
-        const u16x8 one = P::ones();
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int p = PL - 1; p >= 0; --p) {
-            // (a product with 1.0 is exact: the sum of the pieces is the column's sum)
-            if constexpr (PL == 1) acc_b[b] = P::mfma(&one, &fg[b][p], acc_b[b]);
-            else acc_b[b] = Bf::mfma(one, fg[b][p], acc_b[b]);
-          }
+          for (int p = PL - 1; p >= 0; --p) bias_sum[b] += P::sum(fg[b][p]);
       }
     }
   }
@@ -507,13 +508,14 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_kernel(
   const int64_t size = (int64_t)n_out * n_in;
   if (whole) leave(reinterpret_cast<E*>(s_all), dw + it.group * size);
   else leave(reinterpret_cast<float*>(s_all), dw_part + item * size);
-  if (sum_bias && h == 0) {
+  if (sum_bias) {
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
+      const float sum = bias_sum[b] + __shfl_xor(bias_sum[b], 32);
       const int n = n0 + wn * 64 + b * 32 + i;
-      if (n >= n_out) continue;
-      if (whole) db[(int64_t)it.group * n_out + n] = P::from_float(acc_b[b][0]);
-      else db_part[(int64_t)item * n_out + n] = acc_b[b][0];
+      if (h != 0 || n >= n_out) continue;
+      if (whole) db[(int64_t)it.group * n_out + n] = P::from_float(sum);
+      else db_part[(int64_t)item * n_out + n] = sum;
     }
   }
 }
@@ -705,6 +707,7 @@ __global__ __launch_bounds__(2 * ROWS, 2) void rows_direct_kernel(
       for (int q = 0; q < 16; ++q) acc[a][b][q] = 0.f;
   const int i = lane & 31, h = lane >> 5;
   const int wc = wave & 1, wr = wave >> 1;
+  const bool busy = wr * 64 < it.last - it.first;   // (the last tile of a group: no products for rows that are not there)
   unsigned x_at = along_at(s_all, wr * 64 + i, h);
   unsigned w_at = WACROSS ? across_at<COLS>(s_all + ROWS * kDeep, wc * A, lane)
                           : along_at(s_all + ROWS * kDeep, wc * A * 32 + i, h);
@@ -721,6 +724,7 @@ __global__ __launch_bounds__(2 * ROWS, 2) void rows_direct_kernel(
       // the loads of the next step go out in threes: a wave that issues all eight first starts its products late
       constexpr int kFrom = s * 3 < 8 ? s * 3 : 8, kUntil = s * 3 + 3 < 8 ? s * 3 + 3 : 8;
       if (left > 0) issue(next, integral_constant<int, kFrom>(), integral_constant<int, kUntil>());
+      if (!busy) return;
       u16x8 fw[A], fx[2];
       if constexpr (WACROSS) {
         unsigned at[A];
@@ -830,15 +834,14 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_direct_kernel(
     next_rows();
   };
 
-  f32x16 acc[A][2], acc_b[2];
+  f32x16 acc[A][2];
+  float bias_sum[2] = {0.f, 0.f};
 #pragma unroll
   for (int b = 0; b < 2; ++b)
 #pragma unroll
-    for (int q = 0; q < 16; ++q) {
-      acc_b[b][q] = 0.f;
+    for (int q = 0; q < 16; ++q)
 #pragma unroll
       for (int a = 0; a < A; ++a) acc[a][b][q] = 0.f;
-    }
   unsigned g_at[2], x_at[A];
 #pragma unroll
   for (int b = 0; b < 2; ++b) g_at[b] = across_at<kTile>(s_all, wn * 2 + b, lane);
@@ -854,7 +857,10 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_direct_kernel(
         for (int b = 0; b < 2; ++b) acc[a][b] = H::mfma(fx[a], fg[b], acc[a][b]);
       if (sum_bias) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) acc_b[b] = H::mfma(P::ones(), fg[b], acc_b[b]);
+        for (int b = 0; b < 2; ++b) {
+          bias_sum[b] += P::sum(fg[b]);
+          asm volatile("" : "+v"(bias_sum[b]));   // (summed now: the compiler would keep the fragments for later)
+        }
       }
     };
     issue(next);
@@ -916,13 +922,14 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_direct_kernel(
   const int64_t size = (int64_t)n_out * n_in;
   if (whole) leave(s_all, dw + it.group * size);
   else leave(reinterpret_cast<float*>(s_all), dw_part + item * size);
-  if (sum_bias && h == 0) {
+  if (sum_bias) {
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
+      const float sum = bias_sum[b] + __shfl_xor(bias_sum[b], 32);
       const int n = n0 + wn * 64 + b * 32 + i;
-      if (n >= n_out) continue;
-      if (whole) db[(int64_t)it.group * n_out + n] = H::from_float(acc_b[b][0]);
-      else db_part[(int64_t)item * n_out + n] = acc_b[b][0];
+      if (h != 0 || n >= n_out) continue;
+      if (whole) db[(int64_t)it.group * n_out + n] = H::from_float(sum);
+      else db_part[(int64_t)item * n_out + n] = sum;
     }
   }
 }
@@ -1122,12 +1129,16 @@ struct Split {   // of the weight gradient
   int64_t items;
 };
 
-// About 512 workgroups where the rows allow it: two to a CU.
+// Writing and reading an item's partial result costs as much as the products of some 700 rows (16-bit) or 150 (fp32), and
+// two (16-bit) or three workgroups fit on a CU: long items and one round of 256 workgroups for the former, two of 256 for
+// the latter.  (bf16, 32768 ragged rows, 16 groups, 1024 x 1024: 95 us; with twice as many items 126 and 28 to join them.)
 Split split_of(int dtype, int64_t rows, int64_t groups, int n_out, int n_in) {
-  const int64_t tiles = (int64_t)tiles_of(n_out, kTile) * tiles_of(n_in, dtype == PV2_F32 ? kTile : wgrad_cols(n_in));
-  const int64_t want = (512 + tiles - 1) / tiles;
+  const bool full = dtype == PV2_F32;
+  const int64_t tiles = (int64_t)tiles_of(n_out, kTile) * tiles_of(n_in, full ? kTile : wgrad_cols(n_in));
+  const int64_t want = ((full ? 512 : 256) + tiles - 1) / tiles;
   int64_t unit = (rows + want - 1) / want;
-  if (unit < 256) unit = 256;
+  const int64_t least = full ? 256 : 1024;
+  if (unit < least) unit = least;
   unit = (unit + 63) / 64 * 64;
   return {(int)unit, rows / unit + groups};
 }
