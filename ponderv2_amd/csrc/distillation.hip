@@ -7,8 +7,8 @@
 //
 // Bound by memory: the forward pass reads T V logits once - every thread keeps a running maximum and a sum of
 // exponentials relative to it, joined at the end - and the backward pass reads them once more and writes T V gradients.
-// Statistics, probabilities and sums are fp32 (exponents relative to the row's maximum, d = (s - max) log2(e) / tau, so
-// that nothing is lost for large logits); gradients are rounded once, to the logits' type.
+// Statistics, probabilities and sums are fp32, exponents relative to the row's maximum (see exponent() below: nothing is
+// lost for large logits); gradients are rounded once, to the logits' type.
 //   V <= 512       a row per 4 .. 64 lanes of a wave, held in registers;
 //   larger V       a workgroup per row, or - few rows - several per row and a second launch that joins their statistics.
 // Sums over rows are formed from per-workgroup sums in a fixed order: no atomics.
@@ -41,16 +41,33 @@ struct H16 {
   static constexpr int kVec = 8;
 };
 
-struct Stat {   // running maximum and sum of exp2((x - m) c)
+// (x - m) c, the exponent (base 2) of x relative to the maximum m.  One fused multiply-add relative to the rounded m c:
+// every use of the same m has the same error in m c, so it leaves softmax and logarithms alone, and the result has one
+// rounding of its own size.  Masks of the type's lowest value overflow m c, infinities have no difference: for those the
+// difference first, m - m being 0 for a finite m.
+__device__ __forceinline__ bool plain(float m) { return fabsf(m) < 1e30f; }
+__device__ __forceinline__ float exponent_far(float x, float m, float c) {
+  return x == m && fabsf(m) < __builtin_huge_valf() ? 0.f : (x - m) * c;
+}
+__device__ __forceinline__ float exponent(float x, float m, float c) {
+  return plain(m) ? fmaf(x, c, -(m * c)) : exponent_far(x, m, c);
+}
+
+struct Stat {   // running maximum m and sum of exp2(exponent(x, m, c))
   float m, s;
 };
 constexpr float kNegInf = -__builtin_huge_valf();
 
+// the factor of sums relative to `m` when the maximum becomes `to` >= m
+__device__ __forceinline__ float rescale(float m, float to, float c) {
+#pragma clang fp contract(off)   // the difference of the rounded products, as exponent() uses them
+  return m == to ? 1.f : exp2_fast(plain(m) && plain(to) ? m * c - to * c : (m - to) * c);
+}
 __device__ __forceinline__ Stat join(Stat a, Stat b, float c) {
   Stat r;
   r.m = fmaxf(a.m, b.m);
   // a side that saw nothing above -inf has sum 0 (or NaN, which has to stay)
-  r.s = (a.m == r.m ? a.s : a.s * exp2_fast((a.m - r.m) * c)) + (b.m == r.m ? b.s : b.s * exp2_fast((b.m - r.m) * c));
+  r.s = a.s * rescale(a.m, r.m, c) + b.s * rescale(b.m, r.m, c);
   return r;
 }
 
@@ -66,16 +83,19 @@ __device__ __forceinline__ Stat join_wave(Stat a, float c, int width) {
 
 template <int N>
 __device__ __forceinline__ void take(Stat& a, const float* x, float c) {
-  float m = x[0];
+  float m = a.m;
 #pragma unroll
-  for (int j = 1; j < N; ++j) m = fmaxf(m, x[j]);
-  m = fmaxf(m, a.m);
-  float s = a.m == m ? a.s : a.s * exp2_fast((a.m - m) * c);
+  for (int j = 0; j < N; ++j) m = fmaxf(m, x[j]);
+  float s = a.s;
+  if (a.m != m) s *= rescale(a.m, m, c);
+  if (plain(m)) {
+    const float mc = m * c;
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    // (-inf) - (-inf): a row that so far holds only -inf adds nothing
-    const float d = x[j] == m ? (m == -kNegInf ? x[j] - m : 0.f) : x[j] - m;
-    s += (m == kNegInf && x[j] == m) ? 0.f : exp2_fast(d * c);
+    for (int j = 0; j < N; ++j) s += exp2_fast(fmaf(x[j], c, -mc));
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)   // (only -inf so far: nothing to add)
+      s += m == kNegInf && x[j] == m ? 0.f : exp2_fast(exponent_far(x[j], m, c));
   }
   a.m = m;
   a.s = s;
@@ -100,7 +120,7 @@ struct Teacher {   // lists of all rows
 };
 
 // The list of `row`, by `width` lanes (a power of two, aligned): ids[e] (-1: does not count), p[e]; returns whether any
-// entry counts, *log2_sum = log2 of sum exp2((t - *top) c).
+// entry counts, *log2_sum = log2 of sum exp2(exponent(t, *top, c)).
 __device__ __forceinline__ bool read_list(const Teacher& t, int64_t row, int classes, float c, int lane, int width,
                                           int* ids, float* p, float* top, float* log2_sum) {
   float m = kNegInf;
@@ -122,7 +142,7 @@ __device__ __forceinline__ bool read_list(const Teacher& t, int64_t row, int cla
   }
   float s = 0.f;
   for (int e = lane; e < t.k; e += width) {
-    const float x = ids[e] >= 0 ? exp2_fast((p[e] - m) * c) : 0.f;
+    const float x = ids[e] >= 0 ? exp2_fast(exponent(p[e], m, c)) : 0.f;
     s += x;
   }
   for (int d = 1; d < width; d <<= 1) s += __shfl_xor(s, d);
@@ -139,10 +159,10 @@ __device__ __forceinline__ float list_loss(const E* __restrict__ x, int k, int l
   float sum = 0.f;
   for (int e = lane; e < k; e += width) {
     if (ids[e] < 0) continue;
-    const float log_p = (t[e] - t_top) * c - t_log2;
+    const float log_p = exponent(t[e], t_top, c) - t_log2;
     const float p = exp2_fast(log_p);
     const float xv = (float)x[ids[e]];
-    const float log_q = (xv == st.m && st.m != kNegInf && st.m != -kNegInf ? 0.f : (xv - st.m) * c) - s_log2;
+    const float log_q = exponent(xv, st.m, c) - s_log2;
     if (!(p == 0.f)) sum += p * (log_p - log_q);   // 0 log 0 = 0, also where q = 0
   }
   for (int d = 1; d < width; d <<= 1) sum += __shfl_xor(sum, d);
@@ -257,7 +277,7 @@ __global__ __launch_bounds__(kThreads) void small_backward_kernel(const typename
     if (mine) {
       float top, t_log2;
       any = read_list(t, row, V, c, lane, width, ids, p, &top, &t_log2);
-      for (int e = lane; e < t.k; e += width) p[e] = ids[e] >= 0 ? exp2_fast((p[e] - top) * c - t_log2) : 0.f;
+      for (int e = lane; e < t.k; e += width) p[e] = ids[e] >= 0 ? exp2_fast(exponent(p[e], top, c) - t_log2) : 0.f;
       m = stats[2 * row];
       s_log2 = log2_of(stats[2 * row + 1]);
       g = any ? scale(row) : 0.f;
@@ -268,7 +288,7 @@ __global__ __launch_bounds__(kThreads) void small_backward_kernel(const typename
           float d = 0.f;
           if (any) {
             const float v = (float)x[row * ld + col];
-            d = g * exp2_fast((v - m) * c - s_log2);
+            d = g * exp2_fast(exponent(v, m, c) - s_log2);
           }
           dx[row * V + col] = (E)d;
         }
@@ -280,7 +300,7 @@ __global__ __launch_bounds__(kThreads) void small_backward_kernel(const typename
         if (ids[e] < 0) continue;
         const float share = class_share(ids, p, t.k, e);
         if (share < 0.f) continue;
-        const float q = exp2_fast(((float)x[row * ld + ids[e]] - m) * c - s_log2);
+        const float q = exp2_fast(exponent((float)x[row * ld + ids[e]], m, c) - s_log2);
         dx[row * V + ids[e]] = (E)(g * (q - share));
       }
     __syncthreads();
@@ -426,13 +446,14 @@ __global__ __launch_bounds__(kThreads) void row_backward_kernel(const typename T
   __shared__ int s_ids[kMaxTop];
   __shared__ float s_p[kMaxTop];
   __shared__ int s_any;
-  for (int64_t unit = blockIdx.x; unit < rows * splits; unit += gridDim.x) {
+  // last rows first: the forward pass read them last, and what it read last is still in the 256 MB cache
+  for (int64_t unit = rows * splits - 1 - blockIdx.x; unit >= 0; unit -= gridDim.x) {
     const int64_t row = unit / splits, a = (unit % splits) * per_split, b = min((int64_t)V, a + per_split);
     if (threadIdx.x < 64) {
       float top, t_log2;
       const bool any = read_list(t, row, V, c, threadIdx.x, 64, s_ids, s_p, &top, &t_log2);
       for (int e = threadIdx.x; e < t.k; e += 64)
-        s_p[e] = s_ids[e] >= 0 ? exp2_fast((s_p[e] - top) * c - t_log2) : 0.f;
+        s_p[e] = s_ids[e] >= 0 ? exp2_fast(exponent(s_p[e], top, c) - t_log2) : 0.f;
       if (threadIdx.x == 0) s_any = any;
     }
     __syncthreads();
@@ -446,24 +467,29 @@ __global__ __launch_bounds__(kThreads) void row_backward_kernel(const typename T
     } else {
       // x and dx rows share their alignment when both begin alike; else every element is stored by itself
       const bool same = ((uintptr_t)xr % 16) == ((uintptr_t)dr % 16);
-      walk<T, 2>(
-          xr, a, b, [&](int64_t j, float v) { dr[j] = (E)(g * exp2_fast((v - m) * c - s_log2)); },
-          [&](int64_t j, const float* v, auto n) {
-            typedef E VecT __attribute__((ext_vector_type(VN)));
+      auto dense = [&](auto q) {   // q(x): its probability
+        walk<T, 2>(
+            xr, a, b, [&](int64_t j, float v) { dr[j] = (E)(g * q(v)); },
+            [&](int64_t j, const float* v, auto n) {
+              typedef E VecT __attribute__((ext_vector_type(VN)));
 #pragma unroll
-            for (int u = 0; u < decltype(n)::value; ++u) {
-              VecT o;
+              for (int u = 0; u < decltype(n)::value; ++u) {
+                VecT o;
 #pragma unroll
-              for (int i = 0; i < VN; ++i) o[i] = (E)(g * exp2_fast((v[u * VN + i] - m) * c - s_log2));
-              E* at = dr + j + (int64_t)u * kThreads * VN;
-              if (same) {
-                *reinterpret_cast<VecT*>(at) = o;
-              } else {
+                for (int i = 0; i < VN; ++i) o[i] = (E)(g * q(v[u * VN + i]));
+                E* at = dr + j + (int64_t)u * kThreads * VN;
+                if (same) {
+                  *reinterpret_cast<VecT*>(at) = o;
+                } else {
 #pragma unroll
-                for (int i = 0; i < VN; ++i) at[i] = o[i];
+                  for (int i = 0; i < VN; ++i) at[i] = o[i];
+                }
               }
-            }
-          });
+            });
+      };
+      const float mc = m * c;
+      if (plain(m)) dense([&](float v) { return exp2_fast(fmaf(v, c, -mc) - s_log2); });
+      else dense([&](float v) { return exp2_fast(exponent_far(v, m, c) - s_log2); });
     }
     __syncthreads();   // the dense values are written before the listed ones replace them
     if (any)
@@ -472,7 +498,7 @@ __global__ __launch_bounds__(kThreads) void row_backward_kernel(const typename T
         if (id < a || id >= b) continue;
         const float share = class_share(s_ids, s_p, t.k, e);
         if (share < 0.f) continue;
-        const float q = exp2_fast(((float)xr[id] - m) * c - s_log2);
+        const float q = exp2_fast(exponent((float)xr[id], m, c) - s_log2);
         dr[id] = (E)(g * (q - share));
       }
     __syncthreads();

@@ -3,19 +3,23 @@
 //
 // A stable radix sort, least significant digit first, of key(i) = id if 0 <= id < G, else G (so rows without a group
 // come last, in row order).  Digits of up to 10 bits: one pass for G < 1024, two up to 2^20.  A pass is
-//   count    every block's histogram of its 4096 keys (LDS counters),
-//   scan     one block per digit over the blocks' counts,
-//   scatter  every wave walks its 1024 keys in order, 64 at a time; lanes with equal digits find each other by one
-//            ballot per digit bit, and a lane's place is (start of the digit) + (earlier blocks, waves and rounds) +
-//            (equal lanes below it).
-// Nothing depends on the order in which blocks or atomics run.  Up to 4096 rows one workgroup does all passes in LDS
-// in a single launch.
+//   count    every block's histogram of its 1024 to 4096 keys,
+//   scan     one block per digit over the blocks' counts (few counts: every block of the next kernel adds them itself),
+//   scatter  every wave walks its quarter of the block's keys in order, 64 at a time; lanes with equal digits find each
+//            other by one ballot per digit bit, and a lane's place is (start of the digit) + (earlier blocks, waves and
+//            rounds) + (equal lanes below it).
+// Counting goes by the same ballots, one LDS update for all equal lanes: with a handful of groups (or the few frequent
+// ids of a vocabulary) an atomic per key would queue at a handful of addresses.
+// Sums of counts are whole numbers, so nothing depends on the order in which blocks or threads run.  Bound by latency: a pass moves 16 bytes a
+// key, and blocks are as small as keeps 256 CUs busy.  Up to 4096 rows one workgroup does all passes in LDS in a single
+// launch.
 #include "common.h"
 
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTile = 4096;        // keys per block of the multi-block sort
+constexpr int kMaxTile = 4096;     // keys per block of the multi-block sort: 1024, 2048 or 4096
+constexpr int kFewCounts = 8192;   // counts that every block adds up itself
 constexpr int kMaxBits = 10;
 constexpr int kMaxDigits = 1 << kMaxBits;
 constexpr int kSmall = 4096;       // rows that one workgroup sorts in LDS
@@ -75,20 +79,37 @@ struct Source {      // keys of a pass: the caller's ids (first pass) or the pre
   }
 };
 
+// counts[digit] += number of lanes that hold it, for the lanes with `ok`; counts belongs to this wave alone
+__device__ __forceinline__ void count_lanes(volatile int* counts, int digit, int bits, bool ok) {
+  const uint64_t mine = same_digit(digit, bits, __ballot(ok));
+  const int lane = threadIdx.x & 63;
+  if (ok && (mine & ((1ull << lane) - 1)) == 0) counts[digit] += __popcll(mine);
+  __builtin_amdgcn_wave_barrier();
+}
+
+// hist[digit][block], or [block][digit] with `by_block`; ROUNDS of 64 keys per wave
+template <int ROUNDS>
 __global__ __launch_bounds__(kThreads) void count_kernel(Source src, int64_t n, int shift, int bits, int n_blocks,
-                                                         int32_t* __restrict__ hist) {
-  __shared__ int s_count[kMaxDigits];
+                                                         bool by_block, int32_t* __restrict__ hist) {
+  constexpr int kWaves = kThreads / 64;
+  __shared__ int s_count[kWaves][kMaxDigits];
   const int digits = 1 << bits, mask = digits - 1;
-  for (int d = threadIdx.x; d < digits; d += kThreads) s_count[d] = 0;
-  __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kTile;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t base = ((int64_t)blockIdx.x * kWaves + wave) * ROUNDS * 64 + lane;
+  int key[ROUNDS];
 #pragma unroll
-  for (int r = 0; r < kTile / kThreads; ++r) {
-    const int64_t i = base + r * kThreads + threadIdx.x;
-    if (i < n) atomicAdd(&s_count[(src(i) >> shift) & mask], 1);
-  }
+  for (int r = 0; r < ROUNDS; ++r) key[r] = base + r * 64 < n ? src(base + r * 64) : -1;
+  for (int d = lane; d < digits; d += 64) s_count[wave][d] = 0;
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) count_lanes(s_count[wave], (key[r] >> shift) & mask, bits, base + r * 64 < n);
   __syncthreads();
-  for (int d = threadIdx.x; d < digits; d += kThreads) hist[(int64_t)d * n_blocks + blockIdx.x] = s_count[d];
+  for (int d = threadIdx.x; d < digits; d += kThreads) {
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) sum += s_count[w][d];
+    hist[by_block ? (int64_t)blockIdx.x * digits + d : (int64_t)d * n_blocks + blockIdx.x] = sum;
+  }
 }
 
 // one block per digit: hist[d][.] -> its exclusive prefix, totals[d]
@@ -108,7 +129,9 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(int32_t* __restrict__ hi
   if (threadIdx.x == 0) totals[blockIdx.x] = run;
 }
 
-// offsets != nullptr (the sort's only pass): offsets[g] = start of digit g, g <= n_groups
+// offsets != nullptr (the sort's only pass): offsets[g] = start of digit g, g <= n_groups.  totals == nullptr: hist holds
+// the blocks' counts [block][digit], not their prefix.
+template <int ROUNDS>
 __global__ __launch_bounds__(kThreads) void scatter_kernel(Source src, const int32_t* __restrict__ order_in, int64_t n,
                                                            int shift, int bits, int n_blocks,
                                                            const int32_t* __restrict__ hist,
@@ -116,32 +139,57 @@ __global__ __launch_bounds__(kThreads) void scatter_kernel(Source src, const int
                                                            int32_t* __restrict__ keys_out,
                                                            int32_t* __restrict__ order_out,
                                                            int32_t* __restrict__ offsets, int n_groups) {
-  constexpr int kWaves = kThreads / 64, kPerWave = kTile / kWaves, kRounds = kPerWave / 64;
+  constexpr int kWaves = kThreads / 64;
   __shared__ int s_at[kWaves][kMaxDigits];
+  __shared__ int s_before[kMaxDigits], s_total[kMaxDigits];   // of a digit: in earlier blocks, in all blocks
   __shared__ int s_wave[kWaves];
   const int digits = 1 << bits, mask = digits - 1;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int d = threadIdx.x; d < digits * kWaves; d += kThreads) s_at[d / digits][d % digits] = 0;
-  __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kTile + wave * kPerWave + lane;
-  int key[kRounds];
+  const int64_t base = ((int64_t)blockIdx.x * kWaves + wave) * ROUNDS * 64 + lane;
+  int key[ROUNDS], row[ROUNDS];
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
+  for (int r = 0; r < ROUNDS; ++r) {
     const int64_t i = base + r * 64;
     key[r] = i < n ? src(i) : -1;
-    if (i < n) atomicAdd(&s_at[wave][(key[r] >> shift) & mask], 1);
+    row[r] = i < n && order_in ? order_in[i] : (int32_t)i;
   }
+  if (totals) {
+    for (int d = threadIdx.x; d < digits; d += kThreads) {
+      s_before[d] = hist[(int64_t)d * n_blocks + blockIdx.x];
+      s_total[d] = totals[d];
+    }
+  } else {
+    // digits next to each other in the threads; fewer than 256 digits: the blocks split over the threads as well
+    for (int d = threadIdx.x; d < digits; d += kThreads) s_before[d] = s_total[d] = 0;
+    __syncthreads();
+    const int parts = max(1, kThreads / digits);
+    for (int d = threadIdx.x % digits; d < digits; d += kThreads) {
+      int before = 0, all = 0;
+#pragma unroll 8
+      for (int b = threadIdx.x / digits; b < n_blocks; b += parts) {
+        const int c = hist[(int64_t)b * digits + d];
+        all += c;
+        before += b < (int)blockIdx.x ? c : 0;
+      }
+      if (all) atomicAdd(&s_total[d], all);
+      if (before) atomicAdd(&s_before[d], before);
+    }
+  }
+  for (int d = lane; d < digits; d += 64) s_at[wave][d] = 0;
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) count_lanes(s_at[wave], (key[r] >> shift) & mask, bits, base + r * 64 < n);
   __syncthreads();
   // s_at[w][d]: counts -> the place of wave w's first key with digit d
   int start = 0;
   for (int d0 = 0; d0 < digits; d0 += kThreads) {
     const int d = d0 + threadIdx.x;
     int sum;
-    const int before = block_exclusive_scan<kThreads>(d < digits ? totals[d] : 0, s_wave, &sum) + start;
+    const int before = block_exclusive_scan<kThreads>(d < digits ? s_total[d] : 0, s_wave, &sum) + start;
     start += sum;
     if (d < digits) {
       if (offsets && blockIdx.x == 0 && d <= n_groups) offsets[d] = before;
-      int at = before + hist[(int64_t)d * n_blocks + blockIdx.x];
+      int at = before + s_before[d];
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
         const int c = s_at[w][d];
@@ -153,9 +201,8 @@ __global__ __launch_bounds__(kThreads) void scatter_kernel(Source src, const int
   __syncthreads();
   volatile int* my_at = s_at[wave];   // only this wave reads and writes it from here on
 #pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    const int64_t i = base + r * 64;
-    const bool ok = i < n;
+  for (int r = 0; r < ROUNDS; ++r) {
+    const bool ok = base + r * 64 < n;
     const int digit = (key[r] >> shift) & mask;
     const uint64_t mine = same_digit(digit, bits, __ballot(ok));
     const int below = __popcll(mine & ((1ull << lane) - 1));
@@ -165,7 +212,7 @@ __global__ __launch_bounds__(kThreads) void scatter_kernel(Source src, const int
     if (ok && below == 0) my_at[digit] = at + __popcll(mine);
     __builtin_amdgcn_wave_barrier();
     if (ok) {
-      order_out[at] = order_in ? order_in[i] : (int32_t)i;
+      order_out[at] = row[r];
       if (keys_out) keys_out[at] = key[r];
     }
   }
@@ -211,7 +258,7 @@ __global__ __launch_bounds__(kSmallThreads) void small_kernel(Source src, int n,
     __syncthreads();
     for (int r = 0; r < rounds; ++r) {
       const int i = (wave * rounds + r) * 64 + lane;
-      if (i < n) atomicAdd(&s_at[wave][(s_key[cur][i] >> shift) & mask], 1);
+      count_lanes(s_at[wave], i < n ? (s_key[cur][i] >> shift) & mask : 0, bits, i < n);
     }
     __syncthreads();
     int count = 0;
@@ -277,6 +324,8 @@ __global__ __launch_bounds__(64) void offsets_from_counts_kernel(const void* cum
   }
 }
 
+int tile_of(int64_t n) { return n > (1 << 21) ? 4096 : n > (1 << 19) ? 2048 : 1024; }
+
 int bits_for(int64_t n_groups) {   // keys 0 .. n_groups
   int b = 1;
   while (b < 31 && (1ll << b) <= n_groups) ++b;
@@ -290,13 +339,13 @@ extern "C" {
 int64_t pv2_row_groups_workspace_ints(int64_t n, int64_t n_groups) {
   if (n <= 0 || n_groups <= 0) return 1;
   if (n <= kSmall) return n;
-  const int64_t n_blocks = (n + kTile - 1) / kTile;
+  const int64_t n_blocks = (n + tile_of(n) - 1) / tile_of(n);
   return 3 * n + kMaxDigits * (n_blocks + 1);
 }
 
 int pv2_row_groups(const void* index, int index_is_64, int64_t n, int64_t n_groups, int32_t* order, int32_t* offsets,
                    int32_t* sorted_ids, int32_t* workspace, pv2_stream_t stream) {
-  PV2_REQUIRE(offsets && n >= 0 && n < (1ll << 31) - kTile, "row_groups: bad row count");
+  PV2_REQUIRE(offsets && n >= 0 && n < (1ll << 31) - kMaxTile, "row_groups: bad row count");
   PV2_REQUIRE(n_groups >= 1 && n_groups <= (1ll << 30), "row_groups: bad group count");
   PV2_REQUIRE(n == 0 || (index && order && workspace), "row_groups: null pointer");
   hipStream_t s = (hipStream_t)stream;
@@ -314,7 +363,8 @@ int pv2_row_groups(const void* index, int index_is_64, int64_t n, int64_t n_grou
                          (int)n_groups, offsets);
     return pv2::check_launch("row_groups");
   }
-  const int n_blocks = (int)((n + kTile - 1) / kTile);
+  const int tile = tile_of(n);
+  const int n_blocks = (int)((n + tile - 1) / tile);
   const int passes = (key_bits + kMaxBits - 1) / kMaxBits;
   const int bits = (key_bits + passes - 1) / passes;
   int32_t* keys[2] = {workspace, workspace + n};
@@ -327,10 +377,20 @@ int pv2_row_groups(const void* index, int index_is_64, int64_t n, int64_t n_grou
     int32_t* order_out = ((passes - 1 - p) & 1) ? other : order;
     int32_t* keys_out = last ? (sorted_ids ? sorted_ids : passes > 1 ? keys[p & 1] : nullptr) : keys[p & 1];
     const int shift = p * bits, digits = 1 << bits;
-    hipLaunchKernelGGL(count_kernel, dim3(n_blocks), dim3(kThreads), 0, s, src, n, shift, bits, n_blocks, hist);
-    hipLaunchKernelGGL(scan_kernel, dim3(digits), dim3(kThreads), 0, s, hist, n_blocks, totals);
-    hipLaunchKernelGGL(scatter_kernel, dim3(n_blocks), dim3(kThreads), 0, s, src, order_in, n, shift, bits, n_blocks,
-                       hist, totals, keys_out, order_out, passes == 1 ? offsets : nullptr, (int)n_groups);
+    const bool few = (int64_t)digits * n_blocks <= kFewCounts;
+#define PV2_PASS(ROUNDS)                                                                                              \
+  do {                                                                                                                \
+    hipLaunchKernelGGL(count_kernel<ROUNDS>, dim3(n_blocks), dim3(kThreads), 0, s, src, n, shift, bits, n_blocks, few, \
+                       hist);                                                                                         \
+    if (!few) hipLaunchKernelGGL(scan_kernel, dim3(digits), dim3(kThreads), 0, s, hist, n_blocks, totals);             \
+    hipLaunchKernelGGL(scatter_kernel<ROUNDS>, dim3(n_blocks), dim3(kThreads), 0, s, src, order_in, n, shift, bits,    \
+                       n_blocks, hist, few ? nullptr : totals, keys_out, order_out, passes == 1 ? offsets : nullptr,   \
+                       (int)n_groups);                                                                                \
+  } while (0)
+    if (tile == 1024) PV2_PASS(4);
+    else if (tile == 2048) PV2_PASS(8);
+    else PV2_PASS(16);
+#undef PV2_PASS
     src.keys = keys_out;
     order_in = order_out;
   }
@@ -343,7 +403,7 @@ int pv2_row_groups(const void* index, int index_is_64, int64_t n, int64_t n_grou
 int pv2_row_offsets(const void* cumulative, int is_64, int64_t n_groups, int64_t n, int32_t* offsets,
                     pv2_stream_t stream) {
   PV2_REQUIRE(cumulative && offsets, "row_offsets: null pointer");
-  PV2_REQUIRE(n >= 0 && n < (1ll << 31) - kTile && n_groups >= 1 && n_groups <= (1ll << 30), "row_offsets: bad shape");
+  PV2_REQUIRE(n >= 0 && n < (1ll << 31) - kMaxTile && n_groups >= 1 && n_groups <= (1ll << 30), "row_offsets: bad shape");
   hipLaunchKernelGGL(offsets_from_counts_kernel, dim3(1), dim3(64), 0, (hipStream_t)stream, cumulative, is_64,
                      (int)n_groups, n, offsets);
   return pv2::check_launch("row_offsets");

@@ -45,13 +45,16 @@ def test_sizes(dtype, n, rows, c, device):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("kind", ["one", "none", "runs", "heavy"])
+@pytest.mark.parametrize("kind", ["one", "none", "runs", "blocks", "heavy"])
 def test_uneven_classes(dtype, kind, device):
-    """A class of all tokens, no class at all, classes of exactly a piece (128 tokens) and around it, one heavy class."""
+    """A class of all tokens, no class at all, classes of exactly a piece (32 tokens) or a block of them (1024), of
+    multiples and around them, one heavy class."""
     torch.manual_seed(3)
     n = 40007
     index = {"one": torch.full((n,), 4), "none": torch.full((n,), -1),
              "runs": torch.repeat_interleave(torch.arange(9), torch.tensor([128, 128, 127, 1, 129, 256, 257, 1, 300])),
+             "blocks": torch.repeat_interleave(torch.arange(12), torch.tensor(
+                 [32, 31, 1, 33, 31, 64, 832, 1024, 1025, 1023, 1, 3000]))[torch.randperm(7097)],
              "heavy": torch.where(torch.rand(n) < 0.7, torch.tensor(2), torch.randint(0, 5000, (n,)))}[kind]
     check(index.to(device), torch.randn(5000, 40, device=device).to(dtype), -0.5)
 
