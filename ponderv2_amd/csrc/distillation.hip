@@ -90,8 +90,10 @@ __device__ __forceinline__ void take(Stat& a, const float* x, float c) {
   if (a.m != m) s *= rescale(a.m, m, c);
   if (plain(m)) {
     const float mc = m * c;
+    float part[4] = {s, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < N; ++j) s += exp2_fast(fmaf(x[j], c, -mc));
+    for (int j = 0; j < N; ++j) part[j & 3] += exp2_fast(fmaf(x[j], c, -mc));
+    s = (part[0] + part[1]) + (part[2] + part[3]);
   } else {
 #pragma unroll
     for (int j = 0; j < N; ++j)   // (only -inf so far: nothing to add)
@@ -321,15 +323,22 @@ __device__ __forceinline__ void walk(const typename T::type* __restrict__ row, i
   if ((int64_t)threadIdx.x < body - a) one(a + threadIdx.x, (float)row[a + threadIdx.x]);
   const int64_t vecs = (b - body) / V;
   int64_t i = threadIdx.x;
-  for (; i + (UNROLL - 1) * kThreads < vecs; i += UNROLL * kThreads) {
-    VecT t[UNROLL];
+  const VecT* vec = reinterpret_cast<const VecT*>(row + body);
+  VecT t[UNROLL];
+  if (i + (UNROLL - 1) * kThreads < vecs) {
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) t[u] = *reinterpret_cast<const VecT*>(row + body + (i + u * kThreads) * V);
+    for (int u = 0; u < UNROLL; ++u) t[u] = vec[i + u * kThreads];
+  }
+  for (; i + (UNROLL - 1) * kThreads < vecs; i += UNROLL * kThreads) {
     float v[UNROLL * V];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
       for (int j = 0; j < V; ++j) v[u * V + j] = (float)t[u][j];
+    if (i + (2 * UNROLL - 1) * kThreads < vecs) {   // the next vectors are on their way while these are worked on
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) t[u] = vec[i + (UNROLL + u) * kThreads];
+    }
     many(body + i * V, v, std::integral_constant<int, UNROLL>());
   }
   for (; i < vecs; i += kThreads) {
@@ -359,7 +368,7 @@ template <typename T>
 __device__ __forceinline__ Stat row_stat(const typename T::type* __restrict__ row, int64_t a, int64_t b, float c) {
   constexpr int V = T::kVec;
   Stat st = {kNegInf, 0.f};
-  walk<T, 4>(
+  walk<T, 2>(
       row, a, b, [&](int64_t, float v) { take<1>(st, &v, c); },
       [&](int64_t, const float* v, auto n) { take<decltype(n)::value * V>(st, v, c); });
   return join_block(st, c);

@@ -10,9 +10,9 @@ import math
 import torch
 
 from . import _lib
-from .kernels import DTYPE_CODE, _ptr, _require_device, _stream
 from .embedding import rows_contiguous
-from .row_groups import on_device, require_index
+from .kernels import DTYPE_CODE, _require_device
+from .row_groups import launch, once_differentiable_backward, ptr, require_index
 
 MAX_TOP = 1024
 MAX_CLASSES = (1 << 30) - 1
@@ -23,37 +23,38 @@ class _TopkDistillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, index, teacher, temperature, reduction):
         (m, v), k = logits.shape, index.shape[1]
-        L = _lib.lib()
-        new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=logits.device)
-        stats, loss, count = new(m, 2), new(), new()
-        row_loss = new(m) if reduction == "none" else None
-        workspace = new(int(L.pv2_topk_distill_workspace_floats(m, v, k)))
-        with on_device(logits):
-            _lib.check(L.pv2_topk_distill_forward(
-                _ptr(logits), DTYPE_CODE[logits.dtype], m, v, logits.stride(0), _ptr(index),
-                int(index.dtype == torch.int64), index.stride(0), _ptr(teacher), DTYPE_CODE[teacher.dtype],
-                teacher.stride(0), k, temperature, int(reduction == "mean"), _ptr(workspace), _ptr(stats),
-                _ptr(row_loss), _ptr(loss), _ptr(count), _stream(logits)), "pv2_topk_distill_forward")
-        ctx.save_for_backward(logits, index, teacher, stats, count)
+        device = logits.device
+        # the rows' statistics, their number, and scratch
+        saved = torch.empty(2 * m + 1 + _lib.lib().pv2_topk_distill_workspace_floats(m, v, k), dtype=torch.float32,
+                            device=device)
+        loss = torch.empty((), dtype=torch.float32, device=device)
+        row_loss = torch.empty(m, dtype=torch.float32, device=device) if reduction == "none" else None
+        stats = ptr(saved)
+        count = stats + 8 * m
+        launch("pv2_topk_distill_forward", device, ptr(logits), DTYPE_CODE[logits.dtype], m, v, logits.stride(0),
+               ptr(index), index.dtype == torch.int64, index.stride(0), ptr(teacher), DTYPE_CODE[teacher.dtype],
+               teacher.stride(0), k, temperature, reduction == "mean", count + 4, stats, ptr(row_loss), ptr(loss), count)
+        ctx.save_for_backward(logits, index, teacher, saved)
         ctx.how = (temperature, reduction)
         return loss if row_loss is None else row_loss
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable_backward
     def backward(ctx, up):
-        logits, index, teacher, stats, count = ctx.saved_tensors
+        logits, index, teacher, saved = ctx.saved_tensors
         temperature, reduction = ctx.how
         (m, v), k = logits.shape, index.shape[1]
         up = up.contiguous()
         grad = torch.empty((m, v), dtype=logits.dtype, device=logits.device)
-        with on_device(logits):
-            _lib.check(_lib.lib().pv2_topk_distill_backward(
-                _ptr(logits), DTYPE_CODE[logits.dtype], m, v, logits.stride(0), _ptr(index),
-                int(index.dtype == torch.int64), index.stride(0), _ptr(teacher), DTYPE_CODE[teacher.dtype],
-                teacher.stride(0), k, temperature, _ptr(stats), _ptr(up), int(reduction == "none"),
-                _ptr(count) if reduction == "mean" else None, _ptr(grad), _stream(logits)),
-                "pv2_topk_distill_backward")
+        stats = ptr(saved)
+        launch("pv2_topk_distill_backward", logits.device, ptr(logits), DTYPE_CODE[logits.dtype], m, v,
+               logits.stride(0), ptr(index), index.dtype == torch.int64, index.stride(0), ptr(teacher),
+               DTYPE_CODE[teacher.dtype], teacher.stride(0), k, temperature, stats, ptr(up), reduction == "none",
+               stats + 8 * m if reduction == "mean" else None, ptr(grad))
         return grad, None, None, None, None
+
+
+def _rows(t, width):
+    return rows_contiguous(t if t.dim() == 2 else t.reshape(-1, width))
 
 
 def topk_distillation(logits, teacher_index, teacher_logits, temperature=1.0, reduction="mean"):
@@ -83,7 +84,6 @@ def topk_distillation(logits, teacher_index, teacher_logits, temperature=1.0, re
     if logits.numel() == 0:   # no rows: nothing to launch, an exact zero that still carries a gradient
         empty = logits.float().sum(-1)
         return empty if reduction == "none" else empty.sum()
-    loss = _TopkDistillation.apply(
-        rows_contiguous(logits.reshape(-1, v)), rows_contiguous(teacher_index.detach().reshape(-1, k)),
-        rows_contiguous(teacher_logits.detach().reshape(-1, k)), temperature, reduction)
+    loss = _TopkDistillation.apply(_rows(logits, v), _rows(teacher_index, k), _rows(teacher_logits.detach(), k),
+                                   temperature, reduction)
     return loss.reshape(lead) if reduction == "none" else loss

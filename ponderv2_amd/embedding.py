@@ -7,8 +7,8 @@ bits, however often a class repeats."""
 import torch
 
 from . import _lib
-from .kernels import DTYPE_CODE, _ptr, _require_device, _stream
-from .row_groups import MAX_GROUPS, MAX_ROWS, on_device, require_index
+from .kernels import DTYPE_CODE, _require_device
+from .row_groups import MAX_GROUPS, MAX_ROWS, launch, once_differentiable_backward, ptr, require_index
 
 
 class _Embedding(torch.autograd.Function):
@@ -17,29 +17,23 @@ class _Embedding(torch.autograd.Function):
         n, (rows, c) = index.numel(), weight.shape
         y = torch.empty((n, c), dtype=weight.dtype, device=weight.device)
         if n:
-            with on_device(weight):
-                _lib.check(_lib.lib().pv2_embedding_forward(
-                    _ptr(index), int(index.dtype == torch.int64), n, _ptr(weight), DTYPE_CODE[weight.dtype], rows, c,
-                    weight.stride(0), scale, _ptr(y), _stream(weight)), "pv2_embedding_forward")
+            launch("pv2_embedding_forward", weight.device, ptr(index), index.dtype == torch.int64, n, ptr(weight),
+                   DTYPE_CODE[weight.dtype], rows, c, weight.stride(0), scale, ptr(y))
         ctx.save_for_backward(index)
         ctx.table = (rows, c, scale)
         return y
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable_backward
     def backward(ctx, gy):
         index, = ctx.saved_tensors
         rows, c, scale = ctx.table
         n = index.numel()
         gy = rows_contiguous(gy)
-        L = _lib.lib()
-        workspace = torch.empty(int(L.pv2_embedding_backward_workspace_ints(n, rows, c)), dtype=torch.int32,
+        workspace = torch.empty(_lib.lib().pv2_embedding_backward_workspace_ints(n, rows, c), dtype=torch.int32,
                                 device=gy.device)
         gw = torch.empty((rows, c), dtype=gy.dtype, device=gy.device)
-        with on_device(gy):
-            _lib.check(L.pv2_embedding_backward(
-                _ptr(index), int(index.dtype == torch.int64), n, _ptr(gy), DTYPE_CODE[gy.dtype], rows, c,
-                gy.stride(0), scale, _ptr(workspace), _ptr(gw), _stream(gy)), "pv2_embedding_backward")
+        launch("pv2_embedding_backward", gy.device, ptr(index), index.dtype == torch.int64, n, ptr(gy),
+               DTYPE_CODE[gy.dtype], rows, c, gy.stride(0), scale, ptr(workspace), ptr(gw))
         return None, gw, None
 
 

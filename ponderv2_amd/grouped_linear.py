@@ -12,8 +12,8 @@ import torch
 
 from . import _lib
 from .embedding import rows_contiguous
-from .kernels import DTYPE_CODE, _ptr, _require_device, _stream
-from .row_groups import RowGroups, on_device
+from .kernels import DTYPE_CODE, _require_device
+from .row_groups import RowGroups, launch, once_differentiable_backward, ptr
 
 MAX_ROWS = (1 << 30) - 1
 MAX_GROUPS = (1 << 20) - 1
@@ -26,21 +26,17 @@ class _GroupedLinear(torch.autograd.Function):
         (m, k), (g, n, _) = x.shape, weight.shape
         y = torch.empty((m, n), dtype=x.dtype, device=x.device)
         if m:
-            with on_device(x):
-                _lib.check(_lib.lib().pv2_grouped_linear_forward(
-                    _ptr(x), DTYPE_CODE[x.dtype], m, k, x.stride(0), _ptr(weight), weight.stride(0), weight.stride(1),
-                    g, n, _ptr(bias), _ptr(order), _ptr(offsets), _ptr(y), _stream(x)), "pv2_grouped_linear_forward")
+            launch("pv2_grouped_linear_forward", x.device, ptr(x), DTYPE_CODE[x.dtype], m, k, x.stride(0), ptr(weight),
+                   weight.stride(0), weight.stride(1), g, n, ptr(bias), ptr(order), ptr(offsets), ptr(y))
         ctx.save_for_backward(x, weight, order, offsets)
         ctx.has_bias = bias is not None
         return y
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable_backward
     def backward(ctx, gy):
         x, weight, order, offsets = ctx.saved_tensors
         (m, k), (g, n, _) = x.shape, weight.shape
         code, gy = DTYPE_CODE[x.dtype], rows_contiguous(gy)
-        L = _lib.lib()
         new = lambda *shape, dtype=x.dtype: torch.empty(shape, dtype=dtype, device=x.device)
         gx = gw = gb = None
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
@@ -48,20 +44,17 @@ class _GroupedLinear(torch.autograd.Function):
             zeros = lambda *shape: torch.zeros(shape, dtype=x.dtype, device=x.device)
             return (zeros(0, k) if need_x else None, zeros(g, n, k) if need_w else None,
                     zeros(g, n) if need_b else None, None, None)
-        with on_device(x):
-            if need_x:
-                gx = new(m, k)
-                _lib.check(L.pv2_grouped_linear_grad_input(
-                    _ptr(gy), code, m, n, gy.stride(0), _ptr(weight), weight.stride(0), weight.stride(1), g, k,
-                    _ptr(order), _ptr(offsets), _ptr(gx), _stream(x)), "pv2_grouped_linear_grad_input")
-            if need_w or need_b:
-                gw = new(g, n, k)
-                gb = new(g, n) if need_b else None
-                floats = int(L.pv2_grouped_linear_workspace_floats(code, m, g, n, k))
-                workspace = new(floats, dtype=torch.float32) if floats else None
-                _lib.check(L.pv2_grouped_linear_grad_weight(
-                    _ptr(gy), code, m, n, gy.stride(0), _ptr(x), k, x.stride(0), g, _ptr(order), _ptr(offsets),
-                    _ptr(workspace), _ptr(gw), _ptr(gb), _stream(x)), "pv2_grouped_linear_grad_weight")
+        if need_x:
+            gx = new(m, k)
+            launch("pv2_grouped_linear_grad_input", x.device, ptr(gy), code, m, n, gy.stride(0), ptr(weight),
+                   weight.stride(0), weight.stride(1), g, k, ptr(order), ptr(offsets), ptr(gx))
+        if need_w or need_b:
+            gw = new(g, n, k)
+            gb = new(g, n) if need_b else None
+            floats = _lib.lib().pv2_grouped_linear_workspace_floats(code, m, g, n, k)
+            workspace = new(floats, dtype=torch.float32) if floats else None
+            launch("pv2_grouped_linear_grad_weight", x.device, ptr(gy), code, m, n, gy.stride(0), ptr(x), k,
+                   x.stride(0), g, ptr(order), ptr(offsets), ptr(workspace), ptr(gw), ptr(gb))
         return gx, gw if need_w else None, gb, None, None
 
 

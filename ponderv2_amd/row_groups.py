@@ -5,22 +5,45 @@
 ``RowGroups.from_offset(offset, n_rows)`` takes rows that already lie group by group, as the points of a batch do
 (``offset``: cumulative row counts, the ``data_dict["offset"]`` convention).
 """
-import contextlib
-
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .kernels import _ptr, _require_device, _stream
+from .kernels import _raw_stream, _require_device
 
 MAX_ROWS = (1 << 31) - 4097
 MAX_GROUPS = 1 << 30
 
 
-def on_device(t):
-    """Kernels are launched on ``t``'s device, whichever is current."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def launch(name, device, *args):
+    """The entry point ``name`` on the current stream of ``device``, whichever device is current.  Tensors are passed by
+    ``data_ptr()``: these calls are made once per layer and step, and next to a kernel of a few microseconds what the
+    host spends on a call is what it takes."""
+    index = device.index
+    fn = getattr(_lib.lib(), name)
+    stream = _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+    if index == torch.cuda.current_device():
+        status = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, stream)
+    if status:
+        _lib.check(status, name)
+
+
+def ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def once_differentiable_backward(fn):
+    """A Function's backward whose results carry no gradient (``once_differentiable``, entered only where grad mode is on:
+    in an ordinary backward pass it is off already)."""
+    strict = once_differentiable(fn)
+
+    def backward(ctx, *grads):
+        return strict(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+
+    return staticmethod(backward)
 
 
 def require_index(index, what):
@@ -50,9 +73,7 @@ class RowGroups:
         offset = offset.detach().contiguous()
         n_groups = offset.numel()
         offsets = torch.empty(n_groups + 1, dtype=torch.int32, device=offset.device)
-        with on_device(offset):
-            _lib.check(_lib.lib().pv2_row_offsets(_ptr(offset), int(offset.dtype == torch.int64), n_groups, n_rows,
-                                                  _ptr(offsets), _stream(offset)), "pv2_row_offsets")
+        launch("pv2_row_offsets", offset.device, ptr(offset), offset.dtype == torch.int64, n_groups, n_rows, ptr(offsets))
         return cls(None, offsets, n_rows, n_groups)
 
 
@@ -67,11 +88,10 @@ def group_rows(index, num_groups):
         raise ValueError(f"group_rows: {n} rows (up to {MAX_ROWS})")
     _require_device(index)
     index = index.detach().contiguous()
-    L = _lib.lib()
-    ints = dict(dtype=torch.int32, device=index.device)
-    order, offsets = torch.empty(n, **ints), torch.empty(num_groups + 1, **ints)
-    workspace = torch.empty(int(L.pv2_row_groups_workspace_ints(n, num_groups)), **ints)
-    with on_device(index):
-        _lib.check(L.pv2_row_groups(_ptr(index), int(index.dtype == torch.int64), n, num_groups, _ptr(order),
-                                    _ptr(offsets), None, _ptr(workspace), _stream(index)), "pv2_row_groups")
+    device = index.device
+    order = torch.empty(n, dtype=torch.int32, device=device)
+    offsets = torch.empty(num_groups + 1, dtype=torch.int32, device=device)
+    workspace = torch.empty(_lib.lib().pv2_row_groups_workspace_ints(n, num_groups), dtype=torch.int32, device=device)
+    launch("pv2_row_groups", device, ptr(index), index.dtype == torch.int64, n, num_groups, ptr(order), ptr(offsets),
+           None, ptr(workspace))
     return RowGroups(order, offsets, n, num_groups)
