@@ -1,7 +1,10 @@
-"""Loss registry with the single criterion the pre-training path touches (PPT's CrossEntropyLoss,
-ponder/models/losses/misc.py:15-40; builder ponder/models/losses/builder.py:13-31)."""
+"""Loss registry with the criterion the pre-training path touches (PPT's CrossEntropyLoss,
+ponder/models/losses/misc.py:15-40; builder ponder/models/losses/builder.py:13-31) and, beside it, distillation from a
+teacher's stored top logits."""
 import torch
 import torch.nn as nn
+
+from ponderv2_amd.distillation import REDUCTIONS, topk_distillation
 
 from ...utils.registry import Registry
 
@@ -23,14 +26,52 @@ class CrossEntropyLoss(nn.Module):
         return self.loss(pred, target) * self.loss_weight
 
 
+@LOSSES.register_module()
+class TopLogitsDistillLoss(nn.Module):
+    """Distillation from a teacher's ``k`` best classes per row (ponderv2_amd/distillation.py): ``target`` is the pair
+    (teacher_index, teacher_logits), (N, k) each, index -1 where a row lists fewer.  ``from_teacher`` tells ``Criteria``
+    to hand it the teacher's lists instead of the labels.  Host tensors and float64 logits take the torch statement."""
+
+    from_teacher = True
+
+    def __init__(self, temperature=1.0, reduction="mean", loss_weight=1.0):
+        super().__init__()
+        assert reduction in REDUCTIONS and temperature > 0
+        self.temperature, self.reduction, self.loss_weight = float(temperature), reduction, loss_weight
+
+    def forward(self, pred, target):
+        index, logits = target
+        if pred.is_cuda and pred.dtype != torch.float64:
+            loss = topk_distillation(pred, index, logits, self.temperature, self.reduction)
+        else:
+            loss = self._statement(pred, index, logits)
+        return loss * self.loss_weight
+
+    def _statement(self, pred, index, logits):
+        t = self.temperature
+        ok = (index >= 0) & (index < pred.shape[-1]) & (logits != -torch.inf)
+        some = ok.any(-1)
+        lists = torch.where(ok, logits.to(pred.dtype) / t, -torch.inf)
+        log_p = torch.log_softmax(torch.where(some[..., None], lists, 0.0), -1)
+        rows = torch.where(some[..., None], pred, 0.0)   # (a row without a list takes no part, whatever it holds)
+        log_q = torch.log_softmax(rows / t, -1).gather(-1, index.long().clamp(0, pred.shape[-1] - 1))
+        p = torch.where(ok, log_p.exp(), 0.0)
+        terms = torch.where(p > 0, p * (torch.where(ok, log_p, 0.0) - log_q), 0.0).sum(-1) * (t * t)
+        terms = torch.where(some, terms, 0.0)
+        if self.reduction == "none":
+            return terms
+        return terms.sum() / some.sum().clamp(min=1) if self.reduction == "mean" else terms.sum()
+
+
 class Criteria:
     def __init__(self, cfg=None):
         self.criteria = [LOSSES.build(cfg=c) for c in (cfg or [])]
 
-    def __call__(self, pred, target):
+    def __call__(self, pred, target, teacher=None):
+        """``teacher``: (index, logits) of the criteria that are taken against a teacher's lists."""
         if not self.criteria:
             return pred  # loss computed inside the model
-        return sum(c(pred, target) for c in self.criteria)
+        return sum(c(pred, teacher if getattr(c, "from_teacher", False) else target) for c in self.criteria)
 
 
 def build_criteria(cfg):

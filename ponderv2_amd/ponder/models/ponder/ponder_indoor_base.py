@@ -490,7 +490,10 @@ class PonderIndoor(nn.Module):
         feat = linear(data_dict["sparse_backbone_feat"], self.proj_head.weight, self.proj_head.bias)
         feat = feat / feat.norm(dim=-1, keepdim=True)
         sim = linear(feat, self._valid_embedding(self._condition_index(data_dict), feat.device))
-        return self.ppt_criteria(self.logit_scale.exp() * sim, data_dict["segment"])
+        # a criterion that is taken against a teacher (losses.TopLogitsDistillLoss) finds its lists, class numbers of
+        # this condition's valid classes, in the batch
+        teacher = ((data_dict["teacher_index"], data_dict["teacher_logits"]) if "teacher_index" in data_dict else None)
+        return self.ppt_criteria(self.logit_scale.exp() * sim, data_dict["segment"], teacher)
 
     def _projection_dtype(self, device):
         """Reduced precision of the dense projection network: ``proj_autocast`` (a dtype name) or
