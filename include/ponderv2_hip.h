@@ -1047,7 +1047,8 @@ int pv2_voxelize_stage2(int64_t n, int64_t n_vox, const uint64_t* uniq_keys, con
  * The stable order of n rows by an integer id: order [n] lists the rows of id 0 in row order, then those of id 1, ..;
  * rows whose id is outside 0 .. n_groups - 1 come last.  The rows of id g are order[offsets[g]] .. order[offsets[g+1] - 1]
  * (offsets [n_groups + 1]).  index: int64 if index_is_64, else int32.  sorted_ids (may be null) [n]: the ids in that
- * order, n_groups for the rows of no group.  workspace: pv2_row_groups_workspace_ints(n, n_groups) ints.
+ * order, n_groups for the rows of no group.  workspace: pv2_row_groups_workspace_ints(n, n_groups) ints (may
+ * be null if that is 0).
  * n < 2^31 - 4096, n_groups <= 2^30.
  * pv2_row_offsets: the same offsets for rows that already lie group by group, from the groups' cumulative row counts
  * [n_groups]; whatever the counts hold, the offsets never decrease and lie within 0 .. n. */

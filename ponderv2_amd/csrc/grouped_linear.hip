@@ -274,6 +274,10 @@ template <class P>
 constexpr int kLds = 2 * P::kPlanes * kTile * P::kDepth > 64 * kOutRow<float> * 2 ? 2 * P::kPlanes * kTile * P::kDepth
                                                                                   : 64 * kOutRow<float> * 2;
 
+// Blocks of 32 columns that a wave computes when `left` columns remain: 96 columns are three of a tile's four.  Waves trade
+// the halves of a tile from one workgroup of a CU to its next (256 CUs), so that no SIMD always has the shorter one.
+__device__ __forceinline__ int blocks_of_32(int left) { return left <= 0 ? 0 : left <= 32 ? 1 : 2; }
+
 // WACROSS: the weights' reduction runs across their rows (dX: W is [reduction, columns]) instead of along them (Y)
 template <class P, bool WACROSS>
 __global__ __launch_bounds__(kThreads, 3) void rows_kernel(
@@ -342,7 +346,8 @@ __global__ __launch_bounds__(kThreads, 3) void rows_kernel(
 #pragma unroll
       for (int q = 0; q < 16; ++q) acc[a][b][q] = 0.f;
   const int i = lane & 31, h = lane >> 5;
-  const int wc = wave & 1, wr = wave >> 1;   // the wave's 64 columns and rows
+  const int wc = (wave ^ (blockIdx.x >> 8)) & 1, wr = wave >> 1;   // the wave's 64 columns and rows
+  const int blocks = blocks_of_32(cols - c0 - wc * 64);
 
   load(0);
   for (int k0 = 0; k0 < depth; k0 += D) {
@@ -361,15 +366,17 @@ __global__ __launch_bounds__(kThreads, 3) void rows_kernel(
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int p = 0; p < PL; ++p) {
-          fx[b][p] = along_fragment<D>(s_x + p * kPlane, wr * 64 + b * 32 + i, 2 * s + h);
-          fw[b][p] = WACROSS ? across_fragment(s_w + p * kPlane, s, wc * 2 + b, lane)
-                             : along_fragment<D>(s_w + p * kPlane, wc * 64 + b * 32 + i, 2 * s + h);
-        }
+        for (int p = 0; p < PL; ++p) fx[b][p] = along_fragment<D>(s_x + p * kPlane, wr * 64 + b * 32 + i, 2 * s + h);
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+      for (int a = 0; a < 2; ++a) {
+        if (a >= blocks) break;
+#pragma unroll
+        for (int p = 0; p < PL; ++p)
+          fw[a][p] = WACROSS ? across_fragment(s_w + p * kPlane, s, wc * 2 + a, lane)
+                             : along_fragment<D>(s_w + p * kPlane, wc * 64 + a * 32 + i, 2 * s + h);
 #pragma unroll
         for (int b = 0; b < 2; ++b) acc[a][b] = P::mfma(fw[a], fx[b], acc[a][b]);
+      }
     }
   }
 
@@ -412,7 +419,8 @@ __global__ __launch_bounds__(kThreads, 3) void wgrad_kernel(
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int n0 = tile / tiles_in * kTile, k0 = tile % tiles_in * kTile;
   const int i = lane & 31, h = lane >> 5;
-  const int wk = wave & 1, wn = wave >> 1;
+  const int wk = (wave ^ (blockIdx.x >> 8)) & 1, wn = wave >> 1;
+  const int blocks = blocks_of_32(n_in - k0 - wk * 64);
   const bool sum_bias = db != nullptr && k0 == 0 && wk == 0;
 
   typename P::Raw rx[U], rg[U];
@@ -464,14 +472,15 @@ __global__ __launch_bounds__(kThreads, 3) void wgrad_kernel(
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int p = 0; p < PL; ++p) {
-          fx[b][p] = across_fragment(s_x + p * kPlane, s, wk * 2 + b, lane);
-          fg[b][p] = across_fragment(s_g + p * kPlane, s, wn * 2 + b, lane);
-        }
+        for (int p = 0; p < PL; ++p) fg[b][p] = across_fragment(s_g + p * kPlane, s, wn * 2 + b, lane);
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+      for (int a = 0; a < 2; ++a) {
+        if (a >= blocks) break;
+#pragma unroll
+        for (int p = 0; p < PL; ++p) fx[a][p] = across_fragment(s_x + p * kPlane, s, wk * 2 + a, lane);
 #pragma unroll
         for (int b = 0; b < 2; ++b) acc[a][b] = P::mfma(fx[a], fg[b], acc[a][b]);
+      }
       if (sum_bias) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)

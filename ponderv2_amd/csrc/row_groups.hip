@@ -324,6 +324,8 @@ __global__ __launch_bounds__(64) void offsets_from_counts_kernel(const void* cum
   }
 }
 
+bool few_offsets(int64_t n_groups) { return n_groups <= 8 * kSmallThreads; }   // more are searched by many blocks
+
 int tile_of(int64_t n) { return n > (1 << 21) ? 4096 : n > (1 << 19) ? 2048 : 1024; }
 
 int bits_for(int64_t n_groups) {   // keys 0 .. n_groups
@@ -337,8 +339,8 @@ int bits_for(int64_t n_groups) {   // keys 0 .. n_groups
 extern "C" {
 
 int64_t pv2_row_groups_workspace_ints(int64_t n, int64_t n_groups) {
-  if (n <= 0 || n_groups <= 0) return 1;
-  if (n <= kSmall) return n;
+  if (n <= 0 || n_groups <= 0) return 0;
+  if (n <= kSmall) return few_offsets(n_groups) ? 0 : n;
   const int64_t n_blocks = (n + tile_of(n) - 1) / tile_of(n);
   return 3 * n + kMaxDigits * (n_blocks + 1);
 }
@@ -347,14 +349,14 @@ int pv2_row_groups(const void* index, int index_is_64, int64_t n, int64_t n_grou
                    int32_t* sorted_ids, int32_t* workspace, pv2_stream_t stream) {
   PV2_REQUIRE(offsets && n >= 0 && n < (1ll << 31) - kMaxTile, "row_groups: bad row count");
   PV2_REQUIRE(n_groups >= 1 && n_groups <= (1ll << 30), "row_groups: bad group count");
-  PV2_REQUIRE(n == 0 || (index && order && workspace), "row_groups: null pointer");
+  PV2_REQUIRE(n == 0 || (index && order), "row_groups: null pointer");
+  PV2_REQUIRE(workspace || pv2_row_groups_workspace_ints(n, n_groups) == 0, "row_groups: no workspace");
   hipStream_t s = (hipStream_t)stream;
   if (n == 0) return pv2::zero_words(offsets, n_groups + 1, s);
   Source src{index, index_is_64, nullptr, (int)n_groups};
   const int key_bits = bits_for(n_groups);
   if (n <= kSmall) {
-    // (many offsets are searched by many blocks)
-    const bool inside = n_groups <= 8 * kSmallThreads;
+    const bool inside = few_offsets(n_groups);
     int32_t* keys = sorted_ids ? sorted_ids : inside ? nullptr : workspace;
     hipLaunchKernelGGL(small_kernel, dim3(1), dim3(kSmallThreads), 0, s, src, (int)n, key_bits, (int)n_groups, keys,
                        order, inside ? offsets : nullptr);

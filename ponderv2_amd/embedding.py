@@ -11,17 +11,21 @@ from .kernels import DTYPE_CODE, _require_device
 from .row_groups import MAX_GROUPS, MAX_ROWS, launch, once_differentiable_backward, ptr, require_index
 
 
+def _lookup(index, weight, scale):
+    n, (rows, c) = index.numel(), weight.shape
+    y = torch.empty((n, c), dtype=weight.dtype, device=weight.device)
+    if n:
+        launch("pv2_embedding_forward", weight.device, ptr(index), index.dtype == torch.int64, n, ptr(weight),
+               DTYPE_CODE[weight.dtype], rows, c, weight.stride(0), scale, ptr(y))
+    return y
+
+
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, index, weight, scale):
-        n, (rows, c) = index.numel(), weight.shape
-        y = torch.empty((n, c), dtype=weight.dtype, device=weight.device)
-        if n:
-            launch("pv2_embedding_forward", weight.device, ptr(index), index.dtype == torch.int64, n, ptr(weight),
-                   DTYPE_CODE[weight.dtype], rows, c, weight.stride(0), scale, ptr(y))
         ctx.save_for_backward(index)
-        ctx.table = (rows, c, scale)
-        return y
+        ctx.table = (*weight.shape, scale)
+        return _lookup(index, weight, scale)
 
     @once_differentiable_backward
     def backward(ctx, gy):
@@ -54,5 +58,8 @@ def embedding(index, weight, scale=1.0):
         raise ValueError(f"embedding: index on {index.device}, weight on {weight.device}")
     if index.numel() > MAX_ROWS or weight.shape[0] > MAX_GROUPS:
         raise ValueError(f"embedding: up to {MAX_ROWS} indices and {MAX_GROUPS} rows")
-    y = _Embedding.apply(index.detach().reshape(-1), rows_contiguous(weight), float(scale))
-    return y.reshape(*index.shape, weight.shape[1])
+    flat = index if index.dim() == 1 and index.is_contiguous() else index.reshape(-1).contiguous()
+    # (a lookup without a gradient - serving - is the launch alone)
+    look = _Embedding.apply if weight.requires_grad and torch.is_grad_enabled() else _lookup
+    y = look(flat, rows_contiguous(weight), float(scale))
+    return y if index.dim() == 1 else y.reshape(*index.shape, weight.shape[1])

@@ -20,17 +20,20 @@ MAX_GROUPS = (1 << 20) - 1
 MAX_WIDTH = (1 << 24) - 1
 
 
+def _products(x, weight, bias, order, offsets):
+    (m, k), (g, n, _) = x.shape, weight.shape
+    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    if m:
+        launch("pv2_grouped_linear_forward", x.device, ptr(x), DTYPE_CODE[x.dtype], m, k, x.stride(0), ptr(weight),
+               weight.stride(0), weight.stride(1), g, n, ptr(bias), ptr(order), ptr(offsets), ptr(y))
+    return y
+
+
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, order, offsets):
-        (m, k), (g, n, _) = x.shape, weight.shape
-        y = torch.empty((m, n), dtype=x.dtype, device=x.device)
-        if m:
-            launch("pv2_grouped_linear_forward", x.device, ptr(x), DTYPE_CODE[x.dtype], m, k, x.stride(0), ptr(weight),
-                   weight.stride(0), weight.stride(1), g, n, ptr(bias), ptr(order), ptr(offsets), ptr(y))
         ctx.save_for_backward(x, weight, order, offsets)
-        ctx.has_bias = bias is not None
-        return y
+        return _products(x, weight, bias, order, offsets)
 
     @once_differentiable_backward
     def backward(ctx, gy):
@@ -84,5 +87,7 @@ def grouped_linear(x, weight, groups, bias=None):
     _require_device(*tensors)
     if any(t.device != x.device for t in tensors + [groups.offsets]):
         raise ValueError("grouped_linear: x, weight, bias and groups are on different devices")
-    return _GroupedLinear.apply(rows_contiguous(x), _weight_rows(weight),
-                                None if bias is None else bias.contiguous(), groups.order, groups.offsets)
+    # (products without a gradient - serving - are the launch alone)
+    form = _GroupedLinear.apply if torch.is_grad_enabled() and any(t.requires_grad for t in tensors) else _products
+    return form(rows_contiguous(x), _weight_rows(weight), None if bias is None else bias.contiguous(), groups.order,
+                groups.offsets)

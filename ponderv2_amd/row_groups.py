@@ -70,7 +70,7 @@ class RowGroups:
         if not 0 <= n_rows <= MAX_ROWS:
             raise ValueError(f"RowGroups.from_offset: {n_rows} rows (0 to {MAX_ROWS})")
         _require_device(offset)
-        offset = offset.detach().contiguous()
+        offset = offset.contiguous()
         n_groups = offset.numel()
         offsets = torch.empty(n_groups + 1, dtype=torch.int32, device=offset.device)
         launch("pv2_row_offsets", offset.device, ptr(offset), offset.dtype == torch.int64, n_groups, n_rows, ptr(offsets))
@@ -87,11 +87,12 @@ def group_rows(index, num_groups):
     if n > MAX_ROWS:
         raise ValueError(f"group_rows: {n} rows (up to {MAX_ROWS})")
     _require_device(index)
-    index = index.detach().contiguous()
+    index = index.contiguous()
     device = index.device
     order = torch.empty(n, dtype=torch.int32, device=device)
     offsets = torch.empty(num_groups + 1, dtype=torch.int32, device=device)
-    workspace = torch.empty(_lib.lib().pv2_row_groups_workspace_ints(n, num_groups), dtype=torch.int32, device=device)
+    ints = _lib.lib().pv2_row_groups_workspace_ints(n, num_groups)
+    workspace = torch.empty(ints, dtype=torch.int32, device=device) if ints else None
     launch("pv2_row_groups", device, ptr(index), index.dtype == torch.int64, n, num_groups, ptr(order), ptr(offsets),
            None, ptr(workspace))
     return RowGroups(order, offsets, n, num_groups)

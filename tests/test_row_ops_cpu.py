@@ -105,6 +105,7 @@ def test_c_entries_refuse_before_they_launch():
     calls = [
         (L.pv2_row_groups, (n, 1, 4, 2, p, p, n, p, n)),
         (L.pv2_row_groups, (p, 1, 4, 0, p, p, n, p, n)),
+        (L.pv2_row_groups, (p, 1, 5000, 2, p, p, n, n, n)),       # no workspace
         (L.pv2_row_groups, (p, 1, (1 << 31) - 4096, 2, p, p, n, p, n)),
         (L.pv2_row_groups, (p, 1, 4, (1 << 30) + 1, p, p, n, p, n)),
         (L.pv2_row_offsets, (n, 1, 2, 4, p, n)),
@@ -133,7 +134,8 @@ def test_c_entries_refuse_before_they_launch():
 
 def test_workspaces_cover_what_is_asked():
     L = _lib.lib()
-    assert L.pv2_row_groups_workspace_ints(0, 5) >= 1
+    assert L.pv2_row_groups_workspace_ints(0, 5) == 0 == L.pv2_row_groups_workspace_ints(4096, 8192)
+    assert L.pv2_row_groups_workspace_ints(4096, 8193) >= 4096
     assert L.pv2_row_groups_workspace_ints(100000, 5) >= 3 * 100000
     assert L.pv2_grouped_linear_workspace_floats(0, 100, 4, 64, 64) == 0          # no group can be split
     # 3 groups of 512 x 96: four 128 x 128 tiles, at most 128 + 3 items
