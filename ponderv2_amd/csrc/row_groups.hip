@@ -6,10 +6,10 @@
 //   count    every block's histogram of its 1024 to 4096 keys,
 //   scan     one block per digit over the blocks' counts (few counts: every block of the next kernel adds them itself),
 //   scatter  every wave walks its quarter of the block's keys in order, 64 at a time; lanes with equal digits find each
-//            other by one ballot per digit bit, and a lane's place is (start of the digit) + (earlier blocks, waves and
-//            rounds) + (equal lanes below it).
-// Counting goes by the same ballots, one LDS update for all equal lanes: with a handful of groups (or the few frequent
-// ids of a vocabulary) an atomic per key would queue at a handful of addresses.
+//            other by one ballot per digit bit, and a lane's place is (start of the digit) + (earlier blocks and waves) +
+//            (earlier rounds and equal lanes below it, known from counting).
+// One LDS update for all equal lanes: with a handful of groups (or the few frequent ids of a vocabulary) an atomic per key
+// would queue at a handful of addresses.
 // Sums of counts are whole numbers, so nothing depends on the order in which blocks or threads run.  Bound by latency: a pass moves 16 bytes a
 // key, and blocks are as small as keeps 256 CUs busy.  Up to 4096 rows one workgroup does all passes in LDS in a single
 // launch.
@@ -79,12 +79,16 @@ struct Source {      // keys of a pass: the caller's ids (first pass) or the pre
   }
 };
 
-// counts[digit] += number of lanes that hold it, for the lanes with `ok`; counts belongs to this wave alone
-__device__ __forceinline__ void count_lanes(volatile int* counts, int digit, int bits, bool ok) {
+// counts[digit] += number of lanes that hold it, for the lanes with `ok`; counts belongs to this wave alone.  Returns how
+// many keys with the digit came before this lane's.
+__device__ __forceinline__ int count_lanes(volatile int* counts, int digit, int bits, bool ok) {
   const uint64_t mine = same_digit(digit, bits, __ballot(ok));
-  const int lane = threadIdx.x & 63;
-  if (ok && (mine & ((1ull << lane) - 1)) == 0) counts[digit] += __popcll(mine);
+  const int below = __popcll(mine & ((1ull << (threadIdx.x & 63)) - 1));
+  const int before = ok ? counts[digit] : 0;
   __builtin_amdgcn_wave_barrier();
+  if (ok && below == 0) counts[digit] = before + __popcll(mine);
+  __builtin_amdgcn_wave_barrier();
+  return before + below;
 }
 
 // hist[digit][block], or [block][digit] with `by_block`; ROUNDS of 64 keys per wave
@@ -146,7 +150,7 @@ __global__ __launch_bounds__(kThreads) void scatter_kernel(Source src, const int
   const int digits = 1 << bits, mask = digits - 1;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t base = ((int64_t)blockIdx.x * kWaves + wave) * ROUNDS * 64 + lane;
-  int key[ROUNDS], row[ROUNDS];
+  int key[ROUNDS], row[ROUNDS], rank[ROUNDS];   // rank: among the wave's keys with the same digit
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
     const int64_t i = base + r * 64;
@@ -178,7 +182,7 @@ __global__ __launch_bounds__(kThreads) void scatter_kernel(Source src, const int
   for (int d = lane; d < digits; d += 64) s_at[wave][d] = 0;
   __builtin_amdgcn_wave_barrier();
 #pragma unroll
-  for (int r = 0; r < ROUNDS; ++r) count_lanes(s_at[wave], (key[r] >> shift) & mask, bits, base + r * 64 < n);
+  for (int r = 0; r < ROUNDS; ++r) rank[r] = count_lanes(s_at[wave], (key[r] >> shift) & mask, bits, base + r * 64 < n);
   __syncthreads();
   // s_at[w][d]: counts -> the place of wave w's first key with digit d
   int start = 0;
@@ -199,22 +203,12 @@ __global__ __launch_bounds__(kThreads) void scatter_kernel(Source src, const int
     }
   }
   __syncthreads();
-  volatile int* my_at = s_at[wave];   // only this wave reads and writes it from here on
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
-    const bool ok = base + r * 64 < n;
-    const int digit = (key[r] >> shift) & mask;
-    const uint64_t mine = same_digit(digit, bits, __ballot(ok));
-    const int below = __popcll(mine & ((1ull << lane) - 1));
-    int at = 0;
-    if (ok) at = my_at[digit] + below;
-    __builtin_amdgcn_wave_barrier();
-    if (ok && below == 0) my_at[digit] = at + __popcll(mine);
-    __builtin_amdgcn_wave_barrier();
-    if (ok) {
-      order_out[at] = row[r];
-      if (keys_out) keys_out[at] = key[r];
-    }
+    if (base + r * 64 >= n) continue;
+    const int at = s_at[wave][(key[r] >> shift) & mask] + rank[r];
+    order_out[at] = row[r];
+    if (keys_out) keys_out[at] = key[r];
   }
 }
 
@@ -256,9 +250,12 @@ __global__ __launch_bounds__(kSmallThreads) void small_kernel(Source src, int n,
     const int bits = min(kSmallBits, key_bits - shift), mask = (1 << bits) - 1;
     for (int d = tid; d < kWaves * kDigits; d += kSmallThreads) s_at[d / kDigits][d % kDigits] = 0;
     __syncthreads();
-    for (int r = 0; r < rounds; ++r) {
+    int rank[kSmall / kSmallThreads];
+#pragma unroll
+    for (int r = 0; r < kSmall / kSmallThreads; ++r) {
       const int i = (wave * rounds + r) * 64 + lane;
-      count_lanes(s_at[wave], i < n ? (s_key[cur][i] >> shift) & mask : 0, bits, i < n);
+      const bool ok = r < rounds && i < n;
+      if (r < rounds) rank[r] = count_lanes(s_at[wave], ok ? (s_key[cur][i] >> shift) & mask : 0, bits, ok);
     }
     __syncthreads();
     int count = 0;
@@ -273,20 +270,11 @@ __global__ __launch_bounds__(kSmallThreads) void small_kernel(Source src, int n,
         at += c;
       }
     __syncthreads();
-    volatile int* my_at = s_at[wave];
-    for (int r = 0; r < rounds; ++r) {
+#pragma unroll
+    for (int r = 0; r < kSmall / kSmallThreads; ++r) {
       const int i = (wave * rounds + r) * 64 + lane;
-      const bool ok = i < n;
-      const int key = ok ? s_key[cur][i] : 0;
-      const int digit = (key >> shift) & mask;
-      const uint64_t mine = same_digit(digit, bits, __ballot(ok));
-      const int below = __popcll(mine & ((1ull << lane) - 1));
-      int place = 0;
-      if (ok) place = my_at[digit] + below;
-      __builtin_amdgcn_wave_barrier();
-      if (ok && below == 0) my_at[digit] = place + __popcll(mine);
-      __builtin_amdgcn_wave_barrier();
-      if (ok) {
+      if (r < rounds && i < n) {
+        const int key = s_key[cur][i], place = s_at[wave][(key >> shift) & mask] + rank[r];
         s_key[cur ^ 1][place] = key;
         s_row[cur ^ 1][place] = s_row[cur][i];
       }
