@@ -663,46 +663,46 @@ __global__ __launch_bounds__(2 * ROWS, 2) void rows_direct_kernel(
     }
     return;
   }
-  // This thread's chunks of a step.  A row past the group repeats the tile's first one and a column past the matrix the
-  // last one: what they give is not written.
-  const u16 *xp[UX], *wp[UW];
+  // This thread's chunks of a step, as bytes from the operands' beginnings: those move on by themselves, and a load takes no
+  // arithmetic.  A row past the group repeats the tile's first one and a column past the matrix the last one: what they
+  // give is not written.
+  unsigned xo[UX], wo[UW];
 #pragma unroll
   for (int u = 0; u < UX; ++u) {
     const int q = tid + u * T, r = s_row[along_row(q)];
-    xp[u] = x + (int64_t)(r >= 0 ? r : s_row[0]) * ldx + along_chunk(q) * 8;
+    xo[u] = (unsigned)(((int64_t)(r >= 0 ? r : s_row[0]) * ldx + along_chunk(q) * 8) * 2);
   }
 #pragma unroll
   for (int u = 0; u < UW; ++u) {
     const int q = tid + u * T;
-    const u16* wg = w + it.group * w_group;
-    wp[u] = WACROSS ? wg + across_row<COLS>(q) * ldw + min(c0 + across_chunk<COLS>(q) * 8, cols - 8)
-                    : wg + min(c0 + along_row(q), cols - 1) * ldw + along_chunk(q) * 8;
+    wo[u] = (unsigned)((WACROSS ? across_row<COLS>(q) * ldw + min(c0 + across_chunk<COLS>(q) * 8, cols - 8)
+                                : min(c0 + along_row(q), cols - 1) * ldw + along_chunk(q) * 8) * 2);
   }
-  const int64_t w_add = WACROSS ? kDeep * ldw : kDeep;
+  const char *xk = reinterpret_cast<const char*>(x), *wk = reinterpret_cast<const char*>(w + it.group * w_group);
+  const int64_t w_add = (WACROSS ? kDeep * ldw : kDeep) * 2;
   int left = depth;   // reduction steps that are not loaded yet
   // chunks FROM .. TO - 1 of the next step: x's, then the weights'
   auto issue = [&](u16* to, auto from, auto until) {
     to += wave * 64 * 8;
     if (left >= kDeep) {
 #pragma unroll
-      for (int u = decltype(from)::value; u < decltype(until)::value; ++u) {
-        if (u < UX) {
-          load_to_lds(xp[u], to + u * T * 8);
-          xp[u] += kDeep;
-        } else {
-          load_to_lds(wp[u - UX], to + u * T * 8);
-          wp[u - UX] += w_add;
-        }
-      }
+      for (int u = decltype(from)::value; u < decltype(until)::value; ++u)
+        load_to_lds((const u16*)(u < UX ? xk + xo[u < UX ? u : 0] : wk + wo[u < UX ? 0 : u - UX]), to + u * T * 8);
     } else {   // the last, shorter step: zeros past the end
       const u16* zeros = reinterpret_cast<const u16*>(g_zeros);
 #pragma unroll
       for (int u = decltype(from)::value; u < decltype(until)::value; ++u) {
         const int q = tid + (u < UX ? u : u - UX) * T;
         const int k = u >= UX && WACROSS ? across_row<COLS>(q) : along_chunk(q) * 8;
-        load_to_lds(k < left ? (u < UX ? xp[u < UX ? u : 0] : wp[u < UX ? 0 : u - UX]) : zeros, to + u * T * 8);
+        load_to_lds(k < left ? (const u16*)(u < UX ? xk + xo[u < UX ? u : 0] : wk + wo[u < UX ? 0 : u - UX]) : zeros,
+                    to + u * T * 8);
       }
     }
+  };
+  auto move_on = [&]() {
+    left -= kDeep;
+    xk += kDeep * 2;
+    wk += w_add;
   };
   static_assert(UX * T * 8 == ROWS * kDeep && UX + UW == 8, "");
   using std::integral_constant;
@@ -723,7 +723,7 @@ __global__ __launch_bounds__(2 * ROWS, 2) void rows_direct_kernel(
   int other = kBuffer;   // where the buffer that is not read now begins, from the one that is
   u16* next = s_all;
   issue(next, integral_constant<int, 0>(), integral_constant<int, 8>());
-  left -= kDeep;
+  move_on();
   wait_for_loads<0>();
   barrier();
   for (int k0 = 0; k0 < depth; k0 += kDeep) {
@@ -753,7 +753,7 @@ __global__ __launch_bounds__(2 * ROWS, 2) void rows_direct_kernel(
     quarter(std::integral_constant<int, 1>());
     quarter(std::integral_constant<int, 2>());
     quarter(std::integral_constant<int, 3>());
-    left -= kDeep;
+    move_on();
     x_at += other * 2;
     w_at += other * 2;
     other = -other;
@@ -1109,8 +1109,9 @@ int launch_rows(const void* x, int64_t ldx, const void* w, int64_t w_group, int6
                        tiles, (E*)y);
     return pv2::check_launch("grouped_linear");
   }
+  // 16-byte aligned rows; operands whose bytes 32 bits count
   const bool direct = sizeof(E) == 2 && aligned16(x, ldx, depth, 2) && aligned16(w, ldw, w_group, 2) &&
-                      (!WACROSS || cols % 8 == 0);
+                      (!WACROSS || cols % 8 == 0) && rows * ldx < (1ll << 31) && (WACROSS ? depth : cols) * ldw < (1ll << 31);
   const int size = direct && large_tiles(rows, cols) ? 256 : 128;
   const int tiles = tiles_of(cols, size);
   const int64_t blocks = (most_items(rows, groups, size) + 7) / 8 * 8 * tiles;
