@@ -171,8 +171,17 @@ __device__ __forceinline__ float list_loss(const E* __restrict__ x, int k, int l
   return sum * kLn2;
 }
 
-// the workgroup's rows' losses and their number -> partial[2 blockIdx.x ..]
-__device__ __forceinline__ void block_sums(float loss, float rows, float* __restrict__ partial) {
+struct Totals {   // of all rows: the sum of the losses (mean: over their rows) and the number of rows that count
+  float *loss, *count;
+  int mean;
+  __device__ __forceinline__ void set(float sum, float rows) const {
+    *loss = mean ? sum / fmaxf(rows, 1.f) : sum;
+    *count = rows;
+  }
+};
+
+// the workgroup's rows' losses and their number -> partial[2 blockIdx.x ..], or the totals if there is no other workgroup
+__device__ __forceinline__ void block_sums(float loss, float rows, float* __restrict__ partial, const Totals& all) {
   __shared__ float s_l[kThreads / 64], s_n[kThreads / 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -190,8 +199,12 @@ __device__ __forceinline__ void block_sums(float loss, float rows, float* __rest
       loss += s_l[w];
       rows += s_n[w];
     }
-    partial[2 * (int64_t)blockIdx.x] = loss;
-    partial[2 * (int64_t)blockIdx.x + 1] = rows;
+    if (gridDim.x == 1) {
+      all.set(loss, rows);
+    } else {
+      partial[2 * (int64_t)blockIdx.x] = loss;
+      partial[2 * (int64_t)blockIdx.x + 1] = rows;
+    }
   }
 }
 
@@ -201,7 +214,7 @@ __global__ __launch_bounds__(kThreads) void small_forward_kernel(const typename 
                                                                  int64_t rows, int V, Teacher t, float c, float scale,
                                                                  int width, float* __restrict__ stats,
                                                                  float* __restrict__ row_loss,
-                                                                 float* __restrict__ partial) {
+                                                                 float* __restrict__ partial, Totals all) {
   extern __shared__ float s_list[];   // [rows of the block][k] ids, then logits
   const int per_block = kThreads / width;
   const int lane = threadIdx.x & (width - 1), slot = threadIdx.x / width;
@@ -233,7 +246,7 @@ __global__ __launch_bounds__(kThreads) void small_forward_kernel(const typename 
       row_sum += any ? 1.f : 0.f;
     }
   }
-  block_sums(loss_sum, row_sum, partial);
+  block_sums(loss_sum, row_sum, partial, all);
 }
 
 // what every row's gradient is multiplied by: upstream, tau and the mean's 1 / number of rows
@@ -406,7 +419,7 @@ __global__ __launch_bounds__(kThreads) void row_forward_kernel(const typename T:
                                                                int64_t rows, int V, Teacher t, float c, float scale,
                                                                const float* __restrict__ part, int splits,
                                                                float* __restrict__ stats, float* __restrict__ row_loss,
-                                                               float* __restrict__ partial) {
+                                                               float* __restrict__ partial, Totals all) {
   __shared__ int s_ids[kMaxTop];
   __shared__ float s_t[kMaxTop];
   float loss_sum = 0.f, row_sum = 0.f;
@@ -441,7 +454,7 @@ __global__ __launch_bounds__(kThreads) void row_forward_kernel(const typename T:
       }
     }
   }
-  block_sums(loss_sum, row_sum, partial);
+  block_sums(loss_sum, row_sum, partial, all);
 }
 
 template <typename T>
@@ -514,9 +527,7 @@ __global__ __launch_bounds__(kThreads) void row_backward_kernel(const typename T
   }
 }
 
-// the sum of the losses (mean: over their rows) and the number of rows that count
-__global__ __launch_bounds__(1024) void totals_kernel(const float* __restrict__ partial, int n, int mean,
-                                                      float* __restrict__ loss_out, float* __restrict__ count_out) {
+__global__ __launch_bounds__(1024) void totals_kernel(const float* __restrict__ partial, int n, Totals all) {
   __shared__ float s_l[16], s_n[16];
   float loss = 0.f, rows = 0.f;
   for (int i = threadIdx.x; i < n; i += 1024) {
@@ -538,8 +549,7 @@ __global__ __launch_bounds__(1024) void totals_kernel(const float* __restrict__ 
       loss += s_l[w];
       rows += s_n[w];
     }
-    *loss_out = mean ? loss / fmaxf(rows, 1.f) : loss;
-    *count_out = rows;
+    all.set(loss, rows);
   }
 }
 
@@ -584,10 +594,11 @@ int forward(const void* x, int64_t ld, int64_t rows, int V, const Teacher& t, fl
   const Plan p = plan_of(rows, V, t.k);
   const float c = kLog2e / tau, scale = tau * tau;
   float* partial = ws;
+  const Totals all = {loss, count, mean};
   if (p.width) {
     hipLaunchKernelGGL((small_forward_kernel<T>), dim3(p.blocks), dim3(kThreads),
                        (size_t)(kThreads / p.width) * t.k * 8, s, (const E*)x, ld, rows, V, t, c, scale, p.width,
-                       stats, row_loss, partial);
+                       stats, row_loss, partial, all);
   } else {
     float* part = nullptr;
     if (p.splits > 1) {
@@ -596,10 +607,9 @@ int forward(const void* x, int64_t ld, int64_t rows, int V, const Teacher& t, fl
                          ld, rows, V, t, c, p.splits, p.per_split, part);
     }
     hipLaunchKernelGGL((row_forward_kernel<T>), dim3(p.blocks), dim3(kThreads), 0, s, (const E*)x, ld, rows, V, t, c,
-                       scale, part, p.splits, stats, row_loss, partial);
+                       scale, part, p.splits, stats, row_loss, partial, all);
   }
-  hipLaunchKernelGGL(totals_kernel, dim3(1), dim3(1024), 0, s, partial, p.blocks, mean, loss,
-                     count);
+  if (p.blocks > 1) hipLaunchKernelGGL(totals_kernel, dim3(1), dim3(1024), 0, s, partial, p.blocks, all);
   return pv2::check_launch("topk_distill_forward");
 }
 
