@@ -1078,7 +1078,8 @@ int pv2_embedding_backward(const void* index, int index_is_64, int64_t n, const 
  *   forward      out [rows, n_out] = x W_g^T + b_g;   grad_input  grad_x [rows, n_in] = grad_out W_g;
  *                rows of no group are zeros in both
  *   grad_weight  grad_weight [groups, n_out, n_in] = grad_out_g^T x_g, grad_bias [groups, n_out] = sum of grad_out_g;
- *                every element written; workspace: pv2_grouped_linear_workspace_floats (may be null if that is 0). */
+ *                every element written; workspace: pv2_grouped_linear_workspace_floats (may be null if that is 0).
+ * At most 4096 groups; rows < 2^30.  order and offsets are not checked. */
 int pv2_grouped_linear_forward(const void* x, int dtype, int64_t rows, int n_in, int64_t x_stride, const void* weight,
                                int64_t weight_group_stride, int64_t weight_row_stride, int64_t groups, int n_out,
                                const void* bias_or_null, const int32_t* order_or_null, const int32_t* offsets,

@@ -1077,7 +1077,7 @@ int64_t most_items(int64_t rows, int64_t groups, int unit) {
   return rows / unit + (rows < groups + 1 ? rows : groups + 1);
 }
 
-constexpr int64_t kMostBlocks = 1 << 24;   // of 256 threads
+constexpr int64_t kMostBlocks = 1 << 24;   // of 256 threads: a grid has fewer than 2^32
 
 // Serving: few rows to a group on average, so that the weights are what is read.
 bool few_rows(int64_t rows, int64_t groups) { return rows <= 16 || rows <= 4 * groups; }
@@ -1115,7 +1115,7 @@ int launch_rows(const void* x, int64_t ldx, const void* w, int64_t w_group, int6
   const int size = direct && large_tiles(rows, cols) ? 256 : 128;
   const int tiles = tiles_of(cols, size);
   const int64_t blocks = (most_items(rows, groups, size) + 7) / 8 * 8 * tiles;
-  PV2_REQUIRE(blocks < kMostBlocks, "grouped_linear: too many tiles");
+  PV2_REQUIRE(blocks < kMostBlocks / (size / 128), "grouped_linear: too many tiles");
   if constexpr (sizeof(E) == 2) {
     if (direct) {
 #define PV2_DIRECT(ROWS, COLS)                                                                                       \
@@ -1190,7 +1190,7 @@ int launch_wgrad(const void* dy, int64_t ldy, const void* x, int64_t ldx, const 
 }
 
 int check_shapes(int64_t rows, int64_t groups, int n_out, int n_in) {
-  PV2_REQUIRE(rows >= 1 && rows < (1ll << 30) && groups >= 1 && groups < (1 << 20), "grouped_linear: bad shape");
+  PV2_REQUIRE(rows >= 1 && rows < (1ll << 30) && groups >= 1 && groups <= 4096, "grouped_linear: bad shape");
   PV2_REQUIRE(n_out >= 1 && n_in >= 1 && n_out < (1 << 24) && n_in < (1 << 24), "grouped_linear: bad shape");
   return PV2_OK;
 }

@@ -7,7 +7,8 @@ are zeros in the result and take no gradient; groups may be empty (their weight 
 
 fp32, bf16 or fp16, one type for x, weight and bias, accumulated in fp32; the gradients (of x, weight and bias, once
 differentiable) are of the same type and summed in a fixed order.  fp32 products are formed from three bf16 pieces per
-operand: an infinity among them gives NaN where fp32 arithmetic would give an infinity."""
+operand (mfma_split.h): an infinity among them may give NaN where fp32 arithmetic would give an infinity, and operands
+below 2^-110 lose low bits.  Up to 4096 groups."""
 import torch
 
 from . import _lib
@@ -16,7 +17,7 @@ from .kernels import DTYPE_CODE, _require_device
 from .row_groups import RowGroups, launch, once_differentiable_backward, ptr
 
 MAX_ROWS = (1 << 30) - 1
-MAX_GROUPS = (1 << 20) - 1
+MAX_GROUPS = 4096   # every workgroup scans the groups' offsets for its own
 MAX_WIDTH = (1 << 24) - 1
 
 

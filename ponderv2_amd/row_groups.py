@@ -53,12 +53,19 @@ def require_index(index, what):
 
 class RowGroups:
     """``order`` int32 (n_rows,), or None where the rows already lie in order: the rows of group 0, of group 1, ..,
-    then the rows of no group; ``offsets`` int32 (n_groups + 1,): where each group's rows begin in it."""
+    then the rows of no group; ``offsets`` int32 (n_groups + 1,): where each group's rows begin in it.  Kernels address
+    memory by both without a check, so they are made here only, by ``group_rows`` and ``from_offset``."""
 
     __slots__ = ("order", "offsets", "n_rows", "n_groups")
 
-    def __init__(self, order, offsets, n_rows, n_groups):
+    def __init__(self, *args, **kwargs):
+        raise TypeError("RowGroups are made by group_rows(index, num_groups) or RowGroups.from_offset(offset, n_rows)")
+
+    @classmethod
+    def _made(cls, order, offsets, n_rows, n_groups):
+        self = object.__new__(cls)
         self.order, self.offsets, self.n_rows, self.n_groups = order, offsets, n_rows, n_groups
+        return self
 
     @classmethod
     def from_offset(cls, offset, n_rows):
@@ -74,7 +81,7 @@ class RowGroups:
         n_groups = offset.numel()
         offsets = torch.empty(n_groups + 1, dtype=torch.int32, device=offset.device)
         launch("pv2_row_offsets", offset.device, ptr(offset), offset.dtype == torch.int64, n_groups, n_rows, ptr(offsets))
-        return cls(None, offsets, n_rows, n_groups)
+        return cls._made(None, offsets, n_rows, n_groups)
 
 
 def group_rows(index, num_groups):
@@ -95,4 +102,4 @@ def group_rows(index, num_groups):
     workspace = torch.empty(ints, dtype=torch.int32, device=device) if ints else None
     launch("pv2_row_groups", device, ptr(index), index.dtype == torch.int64, n, num_groups, ptr(order), ptr(offsets),
            None, ptr(workspace))
-    return RowGroups(order, offsets, n, num_groups)
+    return RowGroups._made(order, offsets, n, num_groups)

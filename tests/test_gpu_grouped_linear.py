@@ -1,5 +1,4 @@
 """grouped_linear() and its gradients on the device against 64-bit products."""
-import numpy as np
 import pytest
 import torch
 
@@ -175,6 +174,41 @@ def test_gradients_that_are_not_needed(device):
         args = [t.detach().requires_grad_(j == i) for j, t in enumerate((x, w, b))]
         got, = torch.autograd.grad(grouped_linear(args[0], args[1], groups, args[2]), args[i], gy)
         assert torch.equal(got, want[i])
+
+
+def test_many_groups(device):
+    """As many groups as there may be, most of them empty; serving and training."""
+    torch.manual_seed(12)
+    for m in (300, 20000):
+        x, w, b, gy = problem(m, 4096, 24, 16, torch.bfloat16, device)
+        check(x, w, ids_of(m, 4096, device), b, gy)
+
+
+def test_a_second_backward_pass_is_refused(device):
+    x = torch.randn(40, 8, device=device, requires_grad=True)
+    w = torch.randn(2, 4, 8, device=device, requires_grad=True)
+    table = torch.randn(5, 8, device=device, requires_grad=True)
+    groups = group_rows(ids_of(40, 2, device), 2)
+    logits = torch.randn(6, 9, device=device, requires_grad=True)
+    index = torch.randint(0, 9, (6, 2), device=device)
+    for out, leaf in ((grouped_linear(x, w, groups).square().sum(), w),
+                      (embedding(torch.tensor([1, 4, 1], device=device), table).square().sum(), table),
+                      (topk_distillation(logits, index, torch.randn(6, 2, device=device)), logits)):
+        first, = torch.autograd.grad(out, leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+            first.square().sum().backward()
+
+
+def test_without_a_gradient_the_results_are_the_same(device):
+    torch.manual_seed(13)
+    x, w, b, _ = problem(500, 3, 40, 24, torch.float16, device)
+    groups = group_rows(ids_of(500, 3, device), 3)
+    leaf = w.clone().requires_grad_()
+    want = grouped_linear(x, leaf, groups, b)
+    with torch.no_grad():
+        assert torch.equal(grouped_linear(x, leaf, groups, b), want)
+    got = grouped_linear(x, w, groups, b)
+    assert torch.equal(got, want) and not got.requires_grad and want.requires_grad
 
 
 def test_no_rows(device):

@@ -19,7 +19,7 @@ def ids(*shape, dtype=torch.int64):
 
 
 def groups_of(n, g):
-    return RowGroups(torch.arange(n, dtype=torch.int32), torch.zeros(g + 1, dtype=torch.int32), n, g)
+    return RowGroups._made(torch.arange(n, dtype=torch.int32), torch.zeros(g + 1, dtype=torch.int32), n, g)
 
 
 def test_host_tensors_are_refused():
@@ -79,6 +79,17 @@ def test_grouped_linear_shapes_and_types():
             grouped_linear(*bad)
 
 
+def test_row_groups_are_not_made_by_hand():
+    """Kernels address memory by their contents."""
+    with pytest.raises(TypeError, match="are made by group_rows"):
+        RowGroups(torch.arange(4, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), 4, 2)
+
+
+def test_grouped_linear_group_limit():
+    with pytest.raises(ValueError, match="4096 groups"):
+        grouped_linear(torch.zeros(4, 1), torch.zeros(4097, 1, 1), groups_of(4, 4097))
+
+
 def test_topk_distillation_arguments():
     s, i, t = torch.zeros(4, 8), ids(4, 2), torch.zeros(4, 2)
     for bad in ((s, i, torch.zeros(4, 3)), (s, ids(3, 2), torch.zeros(3, 2)), (s, ids(2), torch.zeros(2)),
@@ -119,6 +130,7 @@ def test_c_entries_refuse_before_they_launch():
         (L.pv2_grouped_linear_forward, (p, 7, 4, 8, 8, p, 8, 8, 2, 3, n, n, p, p, n)),
         (L.pv2_grouped_linear_forward, (p, 0, 0, 8, 8, p, 8, 8, 2, 3, n, n, p, p, n)),
         (L.pv2_grouped_linear_grad_input, (p, 0, 4, 3, 3, p, 8, 8, 0, 8, n, p, p, n)),
+        (L.pv2_grouped_linear_grad_input, (p, 0, 4, 3, 3, p, 8, 8, 4097, 8, n, p, p, n)),
         (L.pv2_grouped_linear_grad_weight, (p, 0, 4, 3, 3, p, 0, 8, 2, n, p, n, p, n, n)),
         (L.pv2_grouped_linear_grad_weight, (p, 0, 1 << 20, 3, 3, p, 8, 8, 2, n, p, n, p, n, n)),  # no workspace
         (L.pv2_topk_distill_forward, (p, 0, 4, 8, 8, p, 1, 2, p, 0, 2, 1025, 1.0, 0, p, p, n, p, p, n)),
