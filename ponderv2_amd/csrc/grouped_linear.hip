@@ -8,11 +8,27 @@
 // Types: bf16 and fp16 run on their MFMA, fp32 as six bf16 MFMAs over three exact pieces of each operand
 // (mfma_split.h); accumulation is fp32, results are rounded once.
 //
-// rows_kernel      Y and dX: a 128-row x 128-column tile per workgroup, four waves of 64 x 64.
-// wgrad_kernel     dW and db: a 128 x 128 tile of one group's dW; long groups are split over rows into items whose fp32
-//                  partial results a second launch adds in order (no atomics).  db is summed from the fragments of dY.
-// few_rows_kernel  Y for a handful of rows (serving): bound by reading the weights once; 16 output columns per
-//                  workgroup, the reduction split over its four waves, operands straight from memory to registers.
+// rows_kernel          Y and dX: a 128-row x 128-column tile per workgroup, four waves of 64 x 64; fp32, and 16-bit operands
+//                      whose rows are not aligned to 16 bytes.  Operands go through registers (where fp32 is split).
+// rows_direct_kernel   the same for aligned 16-bit operands, memory -> LDS directly: 256 x 256 (waves of 64 x 128) or
+//                      128 x 128.
+// wgrad_kernel,        dW and db: a 128 x 128 (256) tile of one group's dW; long groups are split over rows into items
+// wgrad_direct_kernel  whose fp32 partial results a second launch adds in order (no atomics).  db is summed from the
+//                      fragments of dY.
+// few_rows_kernel      Y for a handful of rows (serving): bound by reading the weights once; 16 output columns per
+//                      workgroup, the reduction split over its four waves, operands straight from memory to registers.
+//
+// Measured on MI355X (a library product of 8192^3 reaches 1374 TFLOP/s in bf16, of 4096^3 137 in fp32):
+//   bf16, 16 groups of 2048 rows, 1024 x 1024   Y 75 us (918 TFLOP/s), dX 80, dW 102; ragged groups 92, 100, 109
+//                                               (one library product of all rows with one weight: 58)
+//   bf16, one group of 32 768, 4096 -> 1024     Y 280 us (983 TFLOP/s)
+//   fp32, the same 16 groups                    Y 365 us (188 TFLOP/s), dX 370, dW 395 (library: 482, 562)
+//   fp32, 3 groups of 92 417 rows, 96 -> 512    Y 77 us, dX 72, dW 81 (library, one weight: 125)
+//   bf16, 8 rows over 16 groups, 1024 -> 2048   9 us (27 MB of weights: 5 us at the rate of a copy)
+// What bounds the 16-bit products: loads into LDS and products overlap only in part.  Alone, with everything else taken out,
+// products take 157 us and loads 196 of the 280 (4096 -> 1024); three stages of 256 x 128 or 32-deep steps three ahead, which
+// wait less but load more, are slower (364 and 350).  The 256 CUs hold 512 tiles of 256 x 256 in two rounds; a few more, as
+// ragged groups make, cost most of a third.
 #include <type_traits>
 
 #include "common.h"
