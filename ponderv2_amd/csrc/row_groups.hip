@@ -12,8 +12,8 @@
 // would queue at a handful of addresses.
 // Sums of counts are whole numbers, so nothing depends on the order in which blocks or threads run.  Bound by latency: a pass moves 16 bytes a
 // key, and blocks are as small as keeps 256 CUs busy.  Up to 4096 rows one workgroup does all passes in LDS in a single
-// launch.  Measured on MI355X: 64 ids 3.4 us; 32 768 ids over 65 536 rows 38 us; 1 000 003 ids over 50 021 groups 62 us
-// (count 9, scan 4, scatter 15 per pass, offsets 7; 12.2 MB at the rate of a copy are 2.4).
+// launch.  Measured on MI355X: 64 ids 3.4 us; 32 768 ids over 65 536 rows 38 us; 1 000 003 ids over 50 021 groups 58 us
+// (count 8, scan 4, scatter 13 per pass, offsets 7; 12.2 MB at the rate of a copy are 2.4).
 #include "common.h"
 
 namespace {
