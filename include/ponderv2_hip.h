@@ -1102,7 +1102,7 @@ int pv2_grouped_linear_grad_weight(const void* grad_out, int dtype, int64_t rows
  *             those rows; row_loss [rows] (may be null); stats [rows, 2] for the backward pass
  *   backward  grad_logits [rows, classes] (contiguous, logits' type) = upstream (one value, or one per row) * d loss_i;
  *             count_or_null: the forward pass's, where it took the mean
- * Strides are in elements, the last axis is contiguous; 1 <= k <= 1024. */
+ * Strides are in elements, the last axis is contiguous; 1 <= k <= 1024, 1e-4 <= T <= 1e4. */
 int64_t pv2_topk_distill_workspace_floats(int64_t rows, int classes, int k);
 int pv2_topk_distill_forward(const void* logits, int dtype, int64_t rows, int classes, int64_t row_stride,
                              const void* teacher_index, int index_is_64, int64_t index_stride,

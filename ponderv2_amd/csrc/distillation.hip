@@ -27,6 +27,7 @@ constexpr int kSmallV = 512;
 constexpr int kPerLane = 8;          // elements of a row that a lane holds (V <= 512)
 constexpr int kMaxTop = 1024;
 constexpr int kSmallLds = 32 * 1024; // teacher entries of a workgroup's rows (V <= 512)
+constexpr float kMinTau = 0.99e-4f, kMaxTau = 1.01e4f;   // (1e-4 .. 1e4, rounded either way)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }  // results below 2^-126: 0
@@ -47,14 +48,17 @@ struct H16 {
 
 // (x - m) c, the exponent (base 2) of x relative to the maximum m.  One fused multiply-add relative to the rounded m c:
 // every use of the same m has the same error in m c, so it leaves softmax and logarithms alone, and the result has one
-// rounding of its own size.  Masks of the type's lowest value overflow m c, infinities have no difference: for those the
-// difference first, m - m being 0 for a finite m.
-__device__ __forceinline__ bool plain(float m) { return fabsf(m) < 1e30f; }
+// rounding of its own size.  That error is at most 1/2 where |m c| < 2^24; larger ones would carry the exponentials past the
+// range of their type (at 2^32 by 2^128), masks of the type's lowest value overflow m c, infinities have no difference: for
+// those the difference first, m - m being 0 for a finite m.
+__device__ __forceinline__ bool plain(float mc) { return fabsf(mc) < 16777216.f; }
 __device__ __forceinline__ float exponent_far(float x, float m, float c) {
   return x == m && fabsf(m) < __builtin_huge_valf() ? 0.f : (x - m) * c;
 }
 __device__ __forceinline__ float exponent(float x, float m, float c) {
-  return plain(m) ? fmaf(x, c, -(m * c)) : exponent_far(x, m, c);
+#pragma clang fp contract(off)   // (the rounded product)
+  const float mc = m * c;
+  return plain(mc) ? fmaf(x, c, -mc) : exponent_far(x, m, c);
 }
 
 struct Stat {   // running maximum m and sum of exp2(exponent(x, m, c))
@@ -62,10 +66,14 @@ struct Stat {   // running maximum m and sum of exp2(exponent(x, m, c))
 };
 constexpr float kNegInf = -__builtin_huge_valf();
 
-// the factor of sums relative to `m` when the maximum becomes `to` >= m
+// the factor of sums relative to `m` when the maximum becomes `to` >= m; relative to m means the rounded m c where that is
+// plain, m c itself elsewhere, as in exponent()
 __device__ __forceinline__ float rescale(float m, float to, float c) {
 #pragma clang fp contract(off)   // the difference of the rounded products, as exponent() uses them
-  return m == to ? 1.f : exp2_fast(plain(m) && plain(to) ? m * c - to * c : (m - to) * c);
+  if (m == to) return 1.f;
+  const float mc = m * c, toc = to * c;
+  const float d = plain(mc) ? (plain(toc) ? mc - toc : fmaf(-to, c, mc)) : plain(toc) ? fmaf(m, c, -toc) : (m - to) * c;
+  return exp2_fast(d);
 }
 __device__ __forceinline__ Stat join(Stat a, Stat b, float c) {
   Stat r;
@@ -92,8 +100,8 @@ __device__ __forceinline__ void take(Stat& a, const float* x, float c) {
   for (int j = 0; j < N; ++j) m = fmaxf(m, x[j]);
   float s = a.s;
   if (a.m != m) s *= rescale(a.m, m, c);
-  if (plain(m)) {
-    const float mc = m * c;
+  const float mc = m * c;
+  if (plain(mc)) {
     float part[4] = {s, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < N; ++j) part[j & 3] += exp2_fast(fmaf(x[j], c, -mc));
@@ -514,7 +522,7 @@ __global__ __launch_bounds__(kThreads) void row_backward_kernel(const typename T
             });
       };
       const float mc = m * c;
-      if (plain(m)) dense([&](float v) { return exp2_fast(fmaf(v, c, -mc) - s_log2); });
+      if (plain(mc)) dense([&](float v) { return exp2_fast(fmaf(v, c, -mc) - s_log2); });
       else dense([&](float v) { return exp2_fast(exponent_far(v, m, c) - s_log2); });
     }
     __syncthreads();   // the dense values are written before the listed ones replace them
@@ -638,7 +646,7 @@ int check_shapes(int64_t rows, int V, int64_t ld, int teacher_dtype, int k, floa
   PV2_REQUIRE(rows > 0 && V > 0 && ld >= 0, "topk_distill: bad shape");
   PV2_REQUIRE(k >= 1 && k <= kMaxTop, "topk_distill: 1 to 1024 listed classes");
   PV2_REQUIRE(teacher_dtype >= PV2_F32 && teacher_dtype <= PV2_F16, "topk_distill: bad element type");
-  PV2_REQUIRE(tau > 0.f && tau < 3e38f, "topk_distill: the temperature is a positive number");
+  PV2_REQUIRE(tau >= kMinTau && tau <= kMaxTau, "topk_distill: temperature out of range");
   return PV2_OK;
 }
 

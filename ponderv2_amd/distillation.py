@@ -3,10 +3,9 @@ for its k best classes per row only (csrc/distillation.hip).
 
 With temperature T, p = softmax(teacher_logits / T) over a row's listed classes and q = softmax(logits / T) over all:
 ``loss_i = T^2 * sum_e p_e (log p_e - log q_{c_e})``, the Kullback-Leibler divergence scaled so that its gradient keeps its
-size when T changes.  An entry counts if its class is one of the logits' (-1: none) and its logit is above -inf; a row
-without one has loss 0 and gradient 0, whatever its logits hold.  A class may be listed twice."""
-import math
-
+size when T changes (1e-4 <= T <= 1e4; the divergence is summed in fp32, so T^2 scales its rounding too).  An entry counts
+if its class is one of the logits' (-1: none) and its logit is above -inf; a row without one has loss 0 and gradient 0,
+whatever its logits hold.  A class may be listed twice."""
 import torch
 
 from . import _lib
@@ -16,6 +15,7 @@ from .row_groups import launch, once_differentiable_backward, ptr, require_index
 
 MAX_TOP = 1024
 MAX_CLASSES = (1 << 30) - 1
+MIN_TEMPERATURE, MAX_TEMPERATURE = 1e-4, 1e4   # 1 / T and T^2 leave fp32 room for the logits
 REDUCTIONS = ("mean", "sum", "none")
 
 
@@ -64,8 +64,8 @@ def topk_distillation(logits, teacher_index, teacher_logits, temperature=1.0, re
     if reduction not in REDUCTIONS:
         raise ValueError(f"topk_distillation: reduction is one of {REDUCTIONS}, got {reduction!r}")
     temperature = float(temperature)
-    if not 0.0 < temperature < math.inf:
-        raise ValueError(f"topk_distillation: temperature is a positive number, got {temperature}")
+    if not MIN_TEMPERATURE <= temperature <= MAX_TEMPERATURE:
+        raise ValueError(f"topk_distillation: temperature {temperature} ({MIN_TEMPERATURE:g} to {MAX_TEMPERATURE:g})")
     require_index(teacher_index, "topk_distillation: teacher_index")
     for name, t in (("logits", logits), ("teacher_logits", teacher_logits)):
         if t.dtype not in DTYPE_CODE:

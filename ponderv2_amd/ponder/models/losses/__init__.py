@@ -4,7 +4,7 @@ teacher's stored top logits."""
 import torch
 import torch.nn as nn
 
-from ponderv2_amd.distillation import REDUCTIONS, topk_distillation
+from ponderv2_amd.distillation import MAX_TEMPERATURE, MIN_TEMPERATURE, REDUCTIONS, topk_distillation
 
 from ...utils.registry import Registry
 
@@ -36,7 +36,7 @@ class TopLogitsDistillLoss(nn.Module):
 
     def __init__(self, temperature=1.0, reduction="mean", loss_weight=1.0):
         super().__init__()
-        assert reduction in REDUCTIONS and temperature > 0
+        assert reduction in REDUCTIONS and MIN_TEMPERATURE <= temperature <= MAX_TEMPERATURE
         self.temperature, self.reduction, self.loss_weight = float(temperature), reduction, loss_weight
 
     def forward(self, pred, target):

@@ -156,6 +156,39 @@ def test_extreme_values(dtype, v, device):
     assert torch.isnan(rows[4]) and torch.isfinite(rows[[0, 1, 2, 3, 5]]).all()
 
 
+# (x - max) / T where the maximum itself, over T, is far past 2^24: a few classes share the maximum, the others lie some of
+# the type's steps below it.  Temperatures are powers of two, so that the 64-bit side divides exactly.
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v,m", [(25, 70), (513, 9), (4097, 600), (20011, 1)])
+@pytest.mark.parametrize("base,temperature", [(1e9, 1.0), (1e9, 8192.0), (3e12, 1.0), (-1e20, 2.0), (1e25, 2.0 ** -13),
+                                              (4e4, 2.0 ** -13), (-1e10, 64.0)])
+def test_large_logits(dtype, v, m, base, temperature, device):
+    torch.manual_seed(v)
+    step = 2.0 ** (-22 if dtype == torch.float32 else -6)
+    near = lambda *shape: base * (1 + torch.randint(-3, 4, shape, device=device) * step)
+    check(near(m, v).to(dtype), torch.randint(0, v, (m, 5), device=device), near(m, 5).to(dtype), temperature)
+
+
+# maxima on both sides of 2^24 ln 2 in one row, in every order: sums relative to one become relative to the other
+@pytest.mark.parametrize("v,m", [(25, 70), (512, 70), (513, 70), (4097, 9), (20011, 1), (20011, 600)])
+@pytest.mark.parametrize("order", ["random", "up", "down"])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_logits_about_where_products_are_rounded(v, m, order, sign, device):
+    torch.manual_seed(v)
+    logits = sign * (11629079 + torch.randint(-6, 7, (m, v), device=device)).float()
+    if order != "random":
+        logits = logits.sort(1, descending=order == "down").values
+    teacher = sign * (11629079 + torch.randint(-6, 7, (m, 5), device=device)).float()
+    check(logits, torch.randint(0, v, (m, 5), device=device), teacher)
+
+
+@pytest.mark.parametrize("v,m", [(25, 70), (4097, 9)])
+@pytest.mark.parametrize("temperature", [1e-4, 1e4])
+def test_ends_of_the_temperatures(v, m, temperature, device):
+    torch.manual_seed(v)
+    check(*problem(m, v, 5, torch.float32, device, "ragged"), temperature=temperature)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("v", [25, 1003])
 def test_shapes_strides_and_types(dtype, v, device):

@@ -110,6 +110,17 @@ def test_topk_distillation_arguments():
             topk_distillation(*bad)
 
 
+def test_temperatures_out_of_range():
+    s, i, t = torch.zeros(4, 8), ids(4, 2), torch.zeros(4, 2)
+    for temperature in (0.99e-4, 1e-30, 1.01e4, 1e30):
+        with pytest.raises(ValueError, match="0.0001 to 10000"):
+            topk_distillation(s, i, t, temperature=temperature)
+    L, p, n = _lib.lib(), ctypes.c_void_p(64), None
+    for temperature in (1e-30, 1e30, float("nan")):
+        assert L.pv2_topk_distill_forward(p, 0, 4, 8, 8, p, 1, 2, p, 0, 2, 2, temperature, 0, p, p, n, p, p, n) == BADARG
+        assert L.pv2_topk_distill_backward(p, 0, 4, 8, 8, p, 1, 2, p, 0, 2, 2, temperature, p, p, 0, n, p, n) == BADARG
+
+
 def test_c_entries_refuse_before_they_launch():
     """Null pointers, sizes out of range and unknown element types come back as an argument error with a text."""
     L, p, n = _lib.lib(), ctypes.c_void_p(64), None
