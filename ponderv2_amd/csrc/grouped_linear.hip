@@ -1121,13 +1121,12 @@ int launch_rows(const void* x, int64_t ldx, const void* w, int64_t w_group, int6
                 const int32_t* order, const int32_t* offsets, int64_t rows, int64_t groups, int cols, int depth,
                 void* y, hipStream_t s) {
   typedef typename P::E E;
-  if (!WACROSS && few_rows(rows, groups)) {
-    const int tiles = tiles_of(cols, 16);
-    const int64_t blocks = (most_items(rows, groups, 16) + 7) / 8 * 8 * tiles;
-    PV2_REQUIRE(blocks < kMostBlocks, "grouped_linear: too many tiles");
-    hipLaunchKernelGGL((few_rows_kernel<P>), dim3((unsigned)blocks), dim3(kThreads), 0, s, (const E*)x, ldx,
+  const int few_tiles = tiles_of(cols, 16);
+  const int64_t few_blocks = (most_items(rows, groups, 16) + 7) / 8 * 8 * few_tiles;
+  if (!WACROSS && few_rows(rows, groups) && few_blocks < kMostBlocks) {
+    hipLaunchKernelGGL((few_rows_kernel<P>), dim3((unsigned)few_blocks), dim3(kThreads), 0, s, (const E*)x, ldx,
                        (const E*)w, w_group, ldw, (const E*)bias, order, offsets, (int)rows, (int)groups, cols, depth,
-                       tiles, (E*)y);
+                       few_tiles, (E*)y);
     return pv2::check_launch("grouped_linear");
   }
   // 16-byte aligned rows; operands whose bytes 32 bits count

@@ -242,6 +242,20 @@ def test_offsets_past_32_bits(device):
     assert int(y.count_nonzero()) == int(y[rows].count_nonzero())
 
 
+def test_few_rows_of_a_very_wide_layer(device):
+    """More blocks of 16 columns than a grid takes: the larger tiles' work, as for more rows."""
+    torch.manual_seed(17)
+    m, g, k, n = 256, 56, 8, 3400008
+    x = torch.randn(m, k, device=device).bfloat16()
+    w = torch.randn(1, n, k, device=device).bfloat16()
+    index = ids_of(m, g, device)
+    y = grouped_linear(x, w.expand(g, n, k), group_rows(index, g))
+    cols = torch.cat((torch.arange(300, device=device), torch.randint(0, n, (300,), device=device),
+                      torch.arange(n - 300, n, device=device)))
+    want, size = exact(x, w[:, cols], torch.where(index >= 0, torch.zeros_like(index), index), None, None)
+    assert_within(y[:, cols], want["y"], product_bound(want["y"], size["y"], k + 1, x.dtype), "y")
+
+
 def test_in_a_graph_with_eager_work_between(device):
     torch.manual_seed(9)
     x, w, b, gy = problem(3000, 5, 64, 48, torch.bfloat16, device)
