@@ -3,7 +3,7 @@
 //
 // A stable radix sort, least significant digit first, of key(i) = id if 0 <= id < G, else G (so rows without a group
 // come last, in row order).  Digits of up to 10 bits: one pass for G < 1024, two up to 2^20.  A pass is
-//   count    every block's histogram of its 1024 (or 4096) keys,
+//   count    every block's histogram of its 512 to 4096 keys,
 //   scan     one block per digit over the blocks' counts (few counts: every block of the next kernel adds them itself),
 //   scatter  every wave walks its quarter of the block's keys in order, 64 at a time; lanes with equal digits find each
 //            other by one ballot per digit bit, and a lane's place is (start of the digit) + (earlier blocks and waves) +
@@ -12,21 +12,21 @@
 // would queue at a handful of addresses.
 // Sums of counts are whole numbers, so nothing depends on the order in which blocks or threads run.  Bound by latency: a pass moves 16 bytes a
 // key, and blocks are as small as keeps 256 CUs busy.  Up to 4096 rows one workgroup does all passes in LDS in a single
-// launch.  Measured on MI355X: 64 ids 3.4 us; 32 768 ids over 65 536 rows 38 us; 1 000 003 ids over 50 021 groups 58 us
-// (count 8, scan 4, scatter 13 per pass, offsets 7; 12.2 MB at the rate of a copy are 2.4).
+// launch.  Measured on MI355X: 64 ids 3.4 us; 32 768 ids over 65 536 rows 28 us; 1 000 003 ids over 50 021 groups 57 us
+// (count 6.5, scan 4.4, scatter 14.4 per pass, offsets 7; 12.2 MB at the rate of a copy are 2.4).
 #include "common.h"
 
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxTile = 4096;     // keys per block of the multi-block sort: 1024 or 4096
-// counts that every block adds up itself (32768 ids, 16 groups: 10.5 us in all against 13.9 with a scan launch; 92001 ids,
-// 36 groups: 12.3 against 14.2)
+constexpr int kMaxTile = 4096;     // most keys per block of the multi-block sort
+// counts that every block adds up itself (32768 ids, 16 groups, 2048 counts: 7.3 us in all against 9.0 with a scan launch;
+// 131072 ids, 8192 counts: 8.6 against 9.3; 92001 ids, 36 groups, 11520 counts: 10.7 against 9.7)
 constexpr int kFewCounts = 8192;
 constexpr int kMaxBits = 10;
 constexpr int kMaxDigits = 1 << kMaxBits;
-// rows that one workgroup sorts in LDS (256 ids, 16 groups: 3.7 us against 7.6 by many workgroups; 4096 ids, 1000 groups:
-// 10.9 against 16.6)
+// rows that one workgroup sorts in LDS (1500 ids, 16 groups: 5.5 us against 7.0 by many workgroups, 1000 groups: 7.9 against
+// 12.6; 4096 ids, 16 groups: 7.7 against 7.1, 1000 groups: 11.5 against 12.3)
 constexpr int kSmall = 4096;
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallBits = 8;
@@ -96,6 +96,13 @@ __device__ __forceinline__ int count_lanes(volatile int* counts, int digit, int 
   return before + below;
 }
 
+// The block of keys that a workgroup takes.  Workgroups are dealt to the 8 XCDs in turn; each XCD takes a contiguous eighth of
+// the blocks, so that the short runs which neighbouring blocks write for a digit meet in one L2 and leave it as whole lines.
+__device__ __forceinline__ int block_of(int n_blocks) {
+  const int x = blockIdx.x & 7;
+  return x * (n_blocks >> 3) + min(x, n_blocks & 7) + (int)(blockIdx.x >> 3);
+}
+
 // hist[digit][block], or [block][digit] with `by_block`; ROUNDS of 64 keys per wave
 template <int ROUNDS>
 __global__ __launch_bounds__(kThreads) void count_kernel(Source src, int64_t n, int shift, int bits, int n_blocks,
@@ -103,8 +110,8 @@ __global__ __launch_bounds__(kThreads) void count_kernel(Source src, int64_t n, 
   constexpr int kWaves = kThreads / 64;
   __shared__ int s_count[kWaves][kMaxDigits];
   const int digits = 1 << bits, mask = digits - 1;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t base = ((int64_t)blockIdx.x * kWaves + wave) * ROUNDS * 64 + lane;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, block = block_of(n_blocks);
+  const int64_t base = ((int64_t)block * kWaves + wave) * ROUNDS * 64 + lane;
   int key[ROUNDS];
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) key[r] = base + r * 64 < n ? src(base + r * 64) : -1;
@@ -117,7 +124,7 @@ __global__ __launch_bounds__(kThreads) void count_kernel(Source src, int64_t n, 
     int sum = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) sum += s_count[w][d];
-    hist[by_block ? (int64_t)blockIdx.x * digits + d : (int64_t)d * n_blocks + blockIdx.x] = sum;
+    hist[by_block ? (int64_t)block * digits + d : (int64_t)d * n_blocks + block] = sum;
   }
 }
 
@@ -153,8 +160,8 @@ __global__ __launch_bounds__(kThreads) void scatter_kernel(Source src, const int
   __shared__ int s_before[kMaxDigits], s_total[kMaxDigits];   // of a digit: in earlier blocks, in all blocks
   __shared__ int s_wave[kWaves];
   const int digits = 1 << bits, mask = digits - 1;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t base = ((int64_t)blockIdx.x * kWaves + wave) * ROUNDS * 64 + lane;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, block = block_of(n_blocks);
+  const int64_t base = ((int64_t)block * kWaves + wave) * ROUNDS * 64 + lane;
   int key[ROUNDS], row[ROUNDS], rank[ROUNDS];   // rank: among the wave's keys with the same digit
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
@@ -164,7 +171,7 @@ __global__ __launch_bounds__(kThreads) void scatter_kernel(Source src, const int
   }
   if (totals) {
     for (int d = threadIdx.x; d < digits; d += kThreads) {
-      s_before[d] = hist[(int64_t)d * n_blocks + blockIdx.x];
+      s_before[d] = hist[(int64_t)d * n_blocks + block];
       s_total[d] = totals[d];
     }
   } else {
@@ -178,7 +185,7 @@ __global__ __launch_bounds__(kThreads) void scatter_kernel(Source src, const int
       for (int b = threadIdx.x / digits; b < n_blocks; b += parts) {
         const int c = hist[(int64_t)b * digits + d];
         all += c;
-        before += b < (int)blockIdx.x ? c : 0;
+        before += b < block ? c : 0;
       }
       if (all) atomicAdd(&s_total[d], all);
       if (before) atomicAdd(&s_before[d], before);
@@ -197,7 +204,7 @@ __global__ __launch_bounds__(kThreads) void scatter_kernel(Source src, const int
     const int before = block_exclusive_scan<kThreads>(d < digits ? s_total[d] : 0, s_wave, &sum) + start;
     start += sum;
     if (d < digits) {
-      if (offsets && blockIdx.x == 0 && d <= n_groups) offsets[d] = before;
+      if (offsets && block == 0 && d <= n_groups) offsets[d] = before;
       int at = before + s_before[d];
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
@@ -319,8 +326,9 @@ __global__ __launch_bounds__(64) void offsets_from_counts_kernel(const void* cum
 
 bool few_offsets(int64_t n_groups) { return n_groups <= 8 * kSmallThreads; }   // more are searched by many blocks
 
-// (32768 ids, 65536 groups: 38 us with 1024, 65 with 4096; a million, 50021 groups: 63 and 88; four million: 163 and 158)
-int tile_of(int64_t n) { return n > (1 << 21) ? 4096 : 1024; }
+// 512, 1024 or 4096 keys per block.  (32768 ids, 65536 groups: 28 us with 512, 34 with 1024; 262144 ids, 50021 groups: 33 and
+// 36; 1000003: 66 and 58; four million, 1000 groups: 88 with 1024, 72 with 4096)
+int tile_of(int64_t n) { return n > (1 << 21) ? 4096 : n > (1 << 18) ? 1024 : 512; }
 
 int bits_for(int64_t n_groups) {   // keys 0 .. n_groups
   int b = 1;
@@ -383,7 +391,8 @@ int pv2_row_groups(const void* index, int index_is_64, int64_t n, int64_t n_grou
                        n_blocks, hist, few ? nullptr : totals, keys_out, order_out, passes == 1 ? offsets : nullptr,   \
                        (int)n_groups);                                                                                \
   } while (0)
-    if (tile == 1024) PV2_PASS(4);
+    if (tile == 512) PV2_PASS(2);
+    else if (tile == 1024) PV2_PASS(4);
     else PV2_PASS(16);
 #undef PV2_PASS
     src.keys = keys_out;

@@ -47,6 +47,14 @@ def test_int32_shapes_and_strides(device):
         assert np.array_equal(got.order.cpu().numpy(), order) and np.array_equal(got.offsets.cpu().numpy(), offsets)
 
 
+# where blocks of another size begin, with and without a full last block
+@pytest.mark.parametrize("n", [4097, 1 << 18, (1 << 18) + 1, 1 << 21, (1 << 21) + 1])
+@pytest.mark.parametrize("count", [36, 50021])
+def test_sizes_of_blocks(n, count, device):
+    rng = np.random.RandomState(n % 1000 + count)
+    check(rng.randint(-1, count, n), count, device)
+
+
 @pytest.mark.parametrize("count", [1, 5, 2000])
 def test_no_rows(count, device):
     got = group_rows(torch.zeros(0, dtype=torch.int64, device=device), count)
