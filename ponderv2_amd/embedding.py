@@ -8,14 +8,32 @@ import torch
 
 from . import _lib
 from .kernels import DTYPE_CODE, _require_device
-from .row_groups import MAX_GROUPS, MAX_ROWS, launch, once_differentiable_backward, ptr, require_index
+from .row_groups import (MAX_GROUPS, MAX_ROWS, launch, launch_alone, once_differentiable_backward, ptr,
+                         require_index)
 
 
-def _lookup(index, weight, scale):
-    n, (rows, c) = index.numel(), weight.shape
-    y = torch.empty((n, c), dtype=weight.dtype, device=weight.device)
+def _checked(index, weight):
+    """The ids as one list and the table with contiguous rows.  Part of every pass through the operator, so that a replayed
+    trace checks and lays out the tensors of its own call."""
+    require_index(index, "embedding")
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"embedding: weight is (rows, channels), got {tuple(weight.shape)}")
+    if weight.dtype not in DTYPE_CODE:
+        raise TypeError(f"embedding: float32, bfloat16 or float16 weight expected, got {weight.dtype}")
+    _require_device(index, weight)
+    if index.device != weight.device:
+        raise ValueError(f"embedding: index on {index.device}, weight on {weight.device}")
+    if index.numel() > MAX_ROWS or weight.shape[0] > MAX_GROUPS:
+        raise ValueError(f"embedding: up to {MAX_ROWS} indices and {MAX_GROUPS} rows")
+    flat = index if index.dim() == 1 and index.is_contiguous() else index.reshape(-1).contiguous()
+    return flat, rows_contiguous(weight)
+
+
+def _lookup(flat, weight, scale, shape):
+    n, (rows, c) = flat.numel(), weight.shape
+    y = torch.empty((*shape, c), dtype=weight.dtype, device=weight.device)
     if n:
-        launch("pv2_embedding_forward", weight.device, ptr(index), index.dtype == torch.int64, n, ptr(weight),
+        launch("pv2_embedding_forward", weight.device, ptr(flat), flat.dtype == torch.int64, n, ptr(weight),
                DTYPE_CODE[weight.dtype], rows, c, weight.stride(0), scale, ptr(y))
     return y
 
@@ -23,16 +41,17 @@ def _lookup(index, weight, scale):
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, index, weight, scale):
-        ctx.save_for_backward(index)
+        flat, weight = _checked(index, weight)
+        ctx.save_for_backward(flat)
         ctx.table = (*weight.shape, scale)
-        return _lookup(index, weight, scale)
+        return _lookup(flat, weight, scale, index.shape)
 
     @once_differentiable_backward
     def backward(ctx, gy):
         index, = ctx.saved_tensors
         rows, c, scale = ctx.table
         n = index.numel()
-        gy = rows_contiguous(gy)
+        gy = rows_contiguous(gy.reshape(-1, c))
         workspace = torch.empty(_lib.lib().pv2_embedding_backward_workspace_ints(n, rows, c), dtype=torch.int32,
                                 device=gy.device)
         gw = torch.empty((rows, c), dtype=gy.dtype, device=gy.device)
@@ -48,18 +67,7 @@ def rows_contiguous(t):
 
 def embedding(index, weight, scale=1.0):
     """index: int64 / int32 ids of any shape; weight (rows, C).  -> (*index.shape, C) = scale * weight[index]."""
-    require_index(index, "embedding")
-    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise ValueError(f"embedding: weight is (rows, channels), got {tuple(weight.shape)}")
-    if weight.dtype not in DTYPE_CODE:
-        raise TypeError(f"embedding: float32, bfloat16 or float16 weight expected, got {weight.dtype}")
-    _require_device(index, weight)
-    if index.device != weight.device:
-        raise ValueError(f"embedding: index on {index.device}, weight on {weight.device}")
-    if index.numel() > MAX_ROWS or weight.shape[0] > MAX_GROUPS:
-        raise ValueError(f"embedding: up to {MAX_ROWS} indices and {MAX_GROUPS} rows")
-    flat = index if index.dim() == 1 and index.is_contiguous() else index.reshape(-1).contiguous()
+    if not launch_alone(weight):
+        return _Embedding.apply(index, weight, float(scale))
     # (a lookup without a gradient - serving - is the launch alone)
-    look = _Embedding.apply if weight.requires_grad and torch.is_grad_enabled() else _lookup
-    y = look(flat, rows_contiguous(weight), float(scale))
-    return y if index.dim() == 1 else y.reshape(*index.shape, weight.shape[1])
+    return _lookup(*_checked(index, weight), float(scale), index.shape)

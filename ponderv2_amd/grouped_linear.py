@@ -14,11 +14,40 @@ import torch
 from . import _lib
 from .embedding import rows_contiguous
 from .kernels import DTYPE_CODE, _require_device
-from .row_groups import RowGroups, launch, once_differentiable_backward, ptr
+from .row_groups import RowGroups, launch, launch_alone, once_differentiable_backward, ptr
 
 MAX_ROWS = (1 << 30) - 1
 MAX_GROUPS = 4096   # every workgroup scans the groups' offsets for its own
 MAX_WIDTH = (1 << 24) - 1
+
+
+def _weight_rows(w):
+    return w if w.stride(2) == 1 or w.shape[2] == 1 else w.contiguous()
+
+
+def _checked(x, weight, bias, order, offsets, n_rows):
+    """The operands with contiguous rows.  Part of every pass through the operator, so that a replayed trace checks and lays
+    out the tensors of its own call.  n_rows: of groups without an order."""
+    if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2]:
+        raise ValueError(f"grouped_linear: x (M, K) and weight (G, N, K) expected, got {tuple(x.shape)} and "
+                         f"{tuple(weight.shape)}")
+    g, n, k = weight.shape
+    n_rows, n_groups = int(n_rows) if order is None else order.numel(), offsets.numel() - 1
+    if n_rows != x.shape[0] or n_groups != g:
+        raise ValueError(f"grouped_linear: {x.shape[0]} rows and {g} weights, but groups of {n_rows} rows in "
+                         f"{n_groups} groups")
+    if bias is not None and tuple(bias.shape) != (g, n):
+        raise ValueError(f"grouped_linear: bias is (G, N) = {(g, n)}, got {tuple(bias.shape)}")
+    if min(n, k) < 1 or max(n, k) > MAX_WIDTH or x.shape[0] > MAX_ROWS or g > MAX_GROUPS:
+        raise ValueError(f"grouped_linear: widths 1 to {MAX_WIDTH}, up to {MAX_ROWS} rows and {MAX_GROUPS} groups")
+    tensors = [x, weight] + ([] if bias is None else [bias])
+    if x.dtype not in DTYPE_CODE or any(t.dtype != x.dtype for t in tensors):
+        raise TypeError("grouped_linear: x, weight and bias are all float32, all bfloat16 or all float16, got "
+                        + ", ".join(str(t.dtype) for t in tensors))
+    _require_device(*tensors)
+    if any(t.device != x.device for t in tensors + [offsets]):
+        raise ValueError("grouped_linear: x, weight, bias and groups are on different devices")
+    return rows_contiguous(x), _weight_rows(weight), None if bias is None else bias.contiguous()
 
 
 def _products(x, weight, bias, order, offsets):
@@ -32,7 +61,8 @@ def _products(x, weight, bias, order, offsets):
 
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, order, offsets):
+    def forward(ctx, x, weight, bias, order, offsets, n_rows):
+        x, weight, bias = _checked(x, weight, bias, order, offsets, n_rows)
         ctx.save_for_backward(x, weight, order, offsets)
         return _products(x, weight, bias, order, offsets)
 
@@ -47,7 +77,7 @@ class _GroupedLinear(torch.autograd.Function):
         if m == 0:
             zeros = lambda *shape: torch.zeros(shape, dtype=x.dtype, device=x.device)
             return (zeros(0, k) if need_x else None, zeros(g, n, k) if need_w else None,
-                    zeros(g, n) if need_b else None, None, None)
+                    zeros(g, n) if need_b else None, None, None, None)
         if need_x:
             gx = new(m, k)
             launch("pv2_grouped_linear_grad_input", x.device, ptr(gy), code, m, n, gy.stride(0), ptr(weight),
@@ -59,36 +89,15 @@ class _GroupedLinear(torch.autograd.Function):
             workspace = new(floats, dtype=torch.float32) if floats else None
             launch("pv2_grouped_linear_grad_weight", x.device, ptr(gy), code, m, n, gy.stride(0), ptr(x), k,
                    x.stride(0), g, ptr(order), ptr(offsets), ptr(workspace), ptr(gw), ptr(gb))
-        return gx, gw if need_w else None, gb, None, None
-
-
-def _weight_rows(w):
-    return w if w.stride(2) == 1 or w.shape[2] == 1 else w.contiguous()
+        return gx, gw if need_w else None, gb, None, None, None
 
 
 def grouped_linear(x, weight, groups, bias=None):
     """x (M, K), weight (G, N, K), groups: RowGroups of M rows in G groups, bias (G, N) or None.  -> (M, N)."""
     if not isinstance(groups, RowGroups):
         raise TypeError("grouped_linear: groups is what row_groups.group_rows or RowGroups.from_offset returns")
-    if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2]:
-        raise ValueError(f"grouped_linear: x (M, K) and weight (G, N, K) expected, got {tuple(x.shape)} and "
-                         f"{tuple(weight.shape)}")
-    g, n, k = weight.shape
-    if groups.n_rows != x.shape[0] or groups.n_groups != g:
-        raise ValueError(f"grouped_linear: {x.shape[0]} rows and {g} weights, but groups of {groups.n_rows} rows in "
-                         f"{groups.n_groups} groups")
-    if bias is not None and tuple(bias.shape) != (g, n):
-        raise ValueError(f"grouped_linear: bias is (G, N) = {(g, n)}, got {tuple(bias.shape)}")
-    if min(n, k) < 1 or max(n, k) > MAX_WIDTH or x.shape[0] > MAX_ROWS or g > MAX_GROUPS:
-        raise ValueError(f"grouped_linear: widths 1 to {MAX_WIDTH}, up to {MAX_ROWS} rows and {MAX_GROUPS} groups")
-    tensors = [x, weight] + ([] if bias is None else [bias])
-    if x.dtype not in DTYPE_CODE or any(t.dtype != x.dtype for t in tensors):
-        raise TypeError("grouped_linear: x, weight and bias are all float32, all bfloat16 or all float16, got "
-                        + ", ".join(str(t.dtype) for t in tensors))
-    _require_device(*tensors)
-    if any(t.device != x.device for t in tensors + [groups.offsets]):
-        raise ValueError("grouped_linear: x, weight, bias and groups are on different devices")
+    order, offsets, n_rows = groups.order, groups.offsets, groups.n_rows
+    if not launch_alone(x, weight, bias):
+        return _GroupedLinear.apply(x, weight, bias, order, offsets, n_rows)
     # (products without a gradient - serving - are the launch alone)
-    form = _GroupedLinear.apply if torch.is_grad_enabled() and any(t.requires_grad for t in tensors) else _products
-    return form(rows_contiguous(x), _weight_rows(weight), None if bias is None else bias.contiguous(), groups.order,
-                groups.offsets)
+    return _products(*_checked(x, weight, bias, order, offsets, n_rows), order, offsets)

@@ -6,6 +6,7 @@
 (``offset``: cumulative row counts, the ``data_dict["offset"]`` convention).
 """
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -33,6 +34,14 @@ def launch(name, device, *args):
 
 def ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def launch_alone(*tensors):
+    """Whether a call may be its launch alone, past the autograd Function: none of ``tensors`` asks for a gradient, none can
+    carry a tangent (the Function refuses those by name) and no trace is recorded (it would keep the empty result and not
+    the launch that fills it)."""
+    return (forward_ad._current_level < 0 and torch._C._get_tracing_state() is None
+            and not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)))
 
 
 def once_differentiable_backward(fn):
