@@ -80,22 +80,25 @@ class RowGroups:
     def from_offset(cls, offset, n_rows):
         """Rows 0 .. offset[0] - 1 are group 0's, offset[0] .. offset[1] - 1 group 1's, ..; rows behind the last
         offset belong to no group."""
-        require_index(offset, "RowGroups.from_offset")
-        if offset.dim() != 1 or offset.numel() < 1:
-            raise ValueError("RowGroups.from_offset: offset is (n_groups,), one group at least")
-        if not 0 <= n_rows <= MAX_ROWS:
-            raise ValueError(f"RowGroups.from_offset: {n_rows} rows (0 to {MAX_ROWS})")
-        _require_device(offset)
-        offset = offset.contiguous()
-        n_groups = offset.numel()
-        offsets = torch.empty(n_groups + 1, dtype=torch.int32, device=offset.device)
-        launch("pv2_row_offsets", offset.device, ptr(offset), offset.dtype == torch.int64, n_groups, n_rows, ptr(offsets))
-        return cls._made(None, offsets, n_rows, n_groups)
+        offsets = _from_offset(offset, n_rows) if launch_alone() else _FromOffset.apply(offset, n_rows)
+        return cls._made(None, offsets, n_rows, offset.numel())
 
 
-def group_rows(index, num_groups):
-    """index: integer ids of the rows (any shape, read as one list).  -> RowGroups with the stable order by id; rows
-    whose id is outside 0 .. num_groups - 1 (padding, unlabelled points at -1) belong to no group."""
+def _from_offset(offset, n_rows):
+    require_index(offset, "RowGroups.from_offset")
+    if offset.dim() != 1 or offset.numel() < 1:
+        raise ValueError("RowGroups.from_offset: offset is (n_groups,), one group at least")
+    if not 0 <= n_rows <= MAX_ROWS:
+        raise ValueError(f"RowGroups.from_offset: {n_rows} rows (0 to {MAX_ROWS})")
+    _require_device(offset)
+    offset = offset.contiguous()
+    n_groups = offset.numel()
+    offsets = torch.empty(n_groups + 1, dtype=torch.int32, device=offset.device)
+    launch("pv2_row_offsets", offset.device, ptr(offset), offset.dtype == torch.int64, n_groups, n_rows, ptr(offsets))
+    return offsets
+
+
+def _group_rows(index, num_groups):
     require_index(index, "group_rows")
     n = index.numel()
     if not 1 <= num_groups <= MAX_GROUPS:
@@ -111,4 +114,24 @@ def group_rows(index, num_groups):
     workspace = torch.empty(ints, dtype=torch.int32, device=device) if ints else None
     launch("pv2_row_groups", device, ptr(index), index.dtype == torch.int64, n, num_groups, ptr(order), ptr(offsets),
            None, ptr(workspace))
-    return RowGroups._made(order, offsets, n, num_groups)
+    return order, offsets
+
+
+# (ids have no gradient: these are what a recorded trace keeps of a call)
+class _FromOffset(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, offset, n_rows):
+        return _from_offset(offset, int(n_rows))
+
+
+class _GroupRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, index, num_groups):
+        return _group_rows(index, int(num_groups))
+
+
+def group_rows(index, num_groups):
+    """index: integer ids of the rows (any shape, read as one list).  -> RowGroups with the stable order by id; rows
+    whose id is outside 0 .. num_groups - 1 (padding, unlabelled points at -1) belong to no group."""
+    order, offsets = (_group_rows if launch_alone() else _GroupRows.apply)(index, num_groups)
+    return RowGroups._made(order, offsets, index.numel(), num_groups)

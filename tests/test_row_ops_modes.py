@@ -155,3 +155,40 @@ def test_traced_products_replay(where):
     assert torch.equal(traced(x, w), products(x, w, index, torch.zeros_like(b)))
     with pytest.raises(Exception, match="groups of 20 rows"):
         traced(torch.cat([x, x]), w)
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_traced_groups_replay(where):
+    """Ids of every replay are sorted anew, for products as well; what is no list of ids is refused."""
+    x, w, b, index = problem(20, 3, 8, 4, where)
+
+    def step(x, w, b, index):
+        groups = group_rows(index, 3)
+        return grouped_linear(x, w, groups, b), groups.order, groups.offsets
+
+    traced = trace(step, x, w, b, index)
+    for m in (20, 33, 1):
+        x, w, b, index = problem(m, 3, 8, 4, where)
+        fill_free_memory(where)
+        y, order, offsets = traced(x, w, b, index)
+        want = group_order(index.cpu().numpy(), 3)
+        assert np.array_equal(order.cpu().numpy(), want[0]) and np.array_equal(offsets.cpu().numpy(), want[1])
+        assert torch.equal(y, products(x, w, index, b))
+    with pytest.raises(Exception, match="group_rows: integer ids"):
+        traced(x, w, b, index.float())
+    with pytest.raises(Exception, match="groups of 2 rows"):
+        traced(x, w, b, index.repeat(2))
+
+    def in_order(x, w, offset):
+        groups = RowGroups.from_offset(offset, x.shape[0])
+        return grouped_linear(x, w, groups), groups.offsets
+
+    x, w, b, _ = problem(20, 3, 8, 4, where)
+    traced = trace(in_order, x, w, torch.tensor([4, 4, 17], device=where))
+    for counts in ([4, 0, 13, 3], [1, 30, 9, 0], [0, 0, 1, 1]):
+        x, w, b, _ = problem(sum(counts), 3, 8, 4, where)
+        index = torch.repeat_interleave(torch.tensor([0, 1, 2, -1]), torch.tensor(counts)).to(where)
+        fill_free_memory(where)
+        y, offsets = traced(x, w, torch.tensor(counts[:3], device=where).cumsum(0))
+        assert offsets.tolist() == [0, *np.cumsum(counts[:3])]
+        assert torch.equal(y, products(x, w, index, torch.zeros_like(b)))
