@@ -19,53 +19,13 @@ MIN_TEMPERATURE, MAX_TEMPERATURE = 1e-4, 1e4   # 1 / T and T^2 leave fp32 room f
 REDUCTIONS = ("mean", "sum", "none")
 
 
-class _TopkDistillation(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, index, teacher, temperature, reduction):
-        (m, v), k = logits.shape, index.shape[1]
-        device = logits.device
-        # the rows' statistics, their number, and scratch
-        saved = torch.empty(2 * m + 1 + _lib.lib().pv2_topk_distill_workspace_floats(m, v, k), dtype=torch.float32,
-                            device=device)
-        loss = torch.empty((), dtype=torch.float32, device=device)
-        row_loss = torch.empty(m, dtype=torch.float32, device=device) if reduction == "none" else None
-        stats = ptr(saved)
-        count = stats + 8 * m
-        launch("pv2_topk_distill_forward", device, ptr(logits), DTYPE_CODE[logits.dtype], m, v, logits.stride(0),
-               ptr(index), index.dtype == torch.int64, index.stride(0), ptr(teacher), DTYPE_CODE[teacher.dtype],
-               teacher.stride(0), k, temperature, reduction == "mean", count + 4, stats, ptr(row_loss), ptr(loss), count)
-        ctx.save_for_backward(logits, index, teacher, saved)
-        ctx.how = (temperature, reduction)
-        return loss if row_loss is None else row_loss
-
-    @once_differentiable_backward
-    def backward(ctx, up):
-        logits, index, teacher, saved = ctx.saved_tensors
-        temperature, reduction = ctx.how
-        (m, v), k = logits.shape, index.shape[1]
-        up = up.contiguous()
-        grad = torch.empty((m, v), dtype=logits.dtype, device=logits.device)
-        stats = ptr(saved)
-        launch("pv2_topk_distill_backward", logits.device, ptr(logits), DTYPE_CODE[logits.dtype], m, v,
-               logits.stride(0), ptr(index), index.dtype == torch.int64, index.stride(0), ptr(teacher),
-               DTYPE_CODE[teacher.dtype], teacher.stride(0), k, temperature, stats, ptr(up), reduction == "none",
-               stats + 8 * m if reduction == "mean" else None, ptr(grad))
-        return grad, None, None, None, None
-
-
 def _rows(t, width):
     return rows_contiguous(t if t.dim() == 2 else t.reshape(-1, width))
 
 
-def topk_distillation(logits, teacher_index, teacher_logits, temperature=1.0, reduction="mean"):
-    """logits (..., V) fp32 / bf16 / fp16; teacher_index (..., k) int64 / int32 and teacher_logits (..., k) fp32 / bf16 /
-    fp16, with the same leading axes.  -> fp32: the mean over the rows that count ("mean", 0 if none does), the sum, or
-    every row's loss ("none").  The gradient, of the logits only, has their type."""
-    if reduction not in REDUCTIONS:
-        raise ValueError(f"topk_distillation: reduction is one of {REDUCTIONS}, got {reduction!r}")
-    temperature = float(temperature)
-    if not MIN_TEMPERATURE <= temperature <= MAX_TEMPERATURE:
-        raise ValueError(f"topk_distillation: temperature {temperature} ({MIN_TEMPERATURE:g} to {MAX_TEMPERATURE:g})")
+def _checked(logits, teacher_index, teacher_logits):
+    """The three as matrices with contiguous rows.  Part of every pass through the operator, so that a replayed trace checks
+    and lays out the tensors of its own call."""
     require_index(teacher_index, "topk_distillation: teacher_index")
     for name, t in (("logits", logits), ("teacher_logits", teacher_logits)):
         if t.dtype not in DTYPE_CODE:
@@ -80,10 +40,57 @@ def topk_distillation(logits, teacher_index, teacher_logits, temperature=1.0, re
     _require_device(logits, teacher_index, teacher_logits)
     if not logits.device == teacher_index.device == teacher_logits.device:
         raise ValueError("topk_distillation: logits, teacher_index and teacher_logits are on different devices")
-    lead = logits.shape[:-1]
-    if logits.numel() == 0:   # no rows: nothing to launch, an exact zero that still carries a gradient
-        empty = logits.float().sum(-1)
-        return empty if reduction == "none" else empty.sum()
-    loss = _TopkDistillation.apply(_rows(logits, v), _rows(teacher_index, k), _rows(teacher_logits.detach(), k),
-                                   temperature, reduction)
-    return loss.reshape(lead) if reduction == "none" else loss
+    return _rows(logits, v), _rows(teacher_index, k), _rows(teacher_logits, k)
+
+
+class _TopkDistillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, index, teacher, temperature, reduction):
+        lead, ctx.dtype = logits.shape[:-1], logits.dtype
+        logits, index, teacher = _checked(logits, index, teacher)
+        m, v, k = int(logits.shape[0]), int(logits.shape[1]), int(index.shape[1])   # (tensors while a trace is recorded)
+        ctx.shape = (*lead, v)
+        device = logits.device
+        if m == 0:   # nothing to launch: an exact zero
+            return torch.zeros(lead if reduction == "none" else (), dtype=torch.float32, device=device)
+        # the rows' statistics, their number, and scratch
+        saved = torch.empty(2 * m + 1 + _lib.lib().pv2_topk_distill_workspace_floats(m, v, k), dtype=torch.float32,
+                            device=device)
+        loss = torch.empty((), dtype=torch.float32, device=device)
+        row_loss = torch.empty(lead, dtype=torch.float32, device=device) if reduction == "none" else None
+        stats = ptr(saved)
+        count = stats + 8 * m
+        launch("pv2_topk_distill_forward", device, ptr(logits), DTYPE_CODE[logits.dtype], m, v, logits.stride(0),
+               ptr(index), index.dtype == torch.int64, index.stride(0), ptr(teacher), DTYPE_CODE[teacher.dtype],
+               teacher.stride(0), k, temperature, reduction == "mean", count + 4, stats, ptr(row_loss), ptr(loss), count)
+        ctx.save_for_backward(logits, index, teacher, saved)
+        ctx.how = (temperature, reduction)
+        return loss if row_loss is None else row_loss
+
+    @once_differentiable_backward
+    def backward(ctx, up):
+        if 0 in ctx.shape:
+            return up.new_zeros(ctx.shape, dtype=ctx.dtype), None, None, None, None
+        logits, index, teacher, saved = ctx.saved_tensors
+        temperature, reduction = ctx.how
+        (m, v), k = logits.shape, index.shape[1]
+        up = up.contiguous()
+        grad = torch.empty((m, v), dtype=logits.dtype, device=logits.device)
+        stats = ptr(saved)
+        launch("pv2_topk_distill_backward", logits.device, ptr(logits), DTYPE_CODE[logits.dtype], m, v,
+               logits.stride(0), ptr(index), index.dtype == torch.int64, index.stride(0), ptr(teacher),
+               DTYPE_CODE[teacher.dtype], teacher.stride(0), k, temperature, stats, ptr(up), reduction == "none",
+               stats + 8 * m if reduction == "mean" else None, ptr(grad))
+        return grad.view(ctx.shape), None, None, None, None
+
+
+def topk_distillation(logits, teacher_index, teacher_logits, temperature=1.0, reduction="mean"):
+    """logits (..., V) fp32 / bf16 / fp16; teacher_index (..., k) int64 / int32 and teacher_logits (..., k) fp32 / bf16 /
+    fp16, with the same leading axes.  -> fp32: the mean over the rows that count ("mean", 0 if none does), the sum, or
+    every row's loss ("none").  The gradient, of the logits only, has their type."""
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"topk_distillation: reduction is one of {REDUCTIONS}, got {reduction!r}")
+    temperature = float(temperature)
+    if not MIN_TEMPERATURE <= temperature <= MAX_TEMPERATURE:
+        raise ValueError(f"topk_distillation: temperature {temperature} ({MIN_TEMPERATURE:g} to {MAX_TEMPERATURE:g})")
+    return _TopkDistillation.apply(logits, teacher_index, teacher_logits.detach(), temperature, reduction)

@@ -8,11 +8,13 @@ import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
-from ponderv2_amd import embedding as embedding_module, grouped_linear as grouped_linear_module, row_groups
+from ponderv2_amd import (_lib, distillation as distillation_module, embedding as embedding_module,
+                          grouped_linear as grouped_linear_module, row_groups)
+from ponderv2_amd.distillation import topk_distillation
 from ponderv2_amd.embedding import embedding
 from ponderv2_amd.grouped_linear import grouped_linear
 from ponderv2_amd.row_groups import RowGroups, group_rows
-from row_ops_oracle import group_order
+from row_ops_oracle import EPS32, distill, group_order
 
 
 def at(address, n, of):
@@ -30,7 +32,9 @@ def matrix_at(address, rows, cols, stride):
 
 def statement(name, device, *args):
     """The entry point ``name`` on host memory, fp32."""
-    args = [int(a) if isinstance(a, torch.Tensor) else a for a in args]   # (sizes while a trace is recorded, as ctypes takes them)
+    for of, a in zip(_lib.SIGNATURES[name][1], args):
+        of.from_param(a)   # what the entry point itself takes
+    args = [int(a) if isinstance(a, torch.Tensor) else a for a in args]   # (sizes while a trace is recorded)
     if name == "pv2_embedding_forward":
         index, is64, n, w, _, rows, c, ldw, scale, y = args
         index = ids_at(index, is64, n)
@@ -56,6 +60,16 @@ def statement(name, device, *args):
         cumulative, is64, count, n, offsets = args
         at(offsets, count + 1, ctypes.c_int32)[:] = np.concatenate(
             [[0], np.maximum.accumulate(ids_at(cumulative, is64, count).clip(0, n))])
+    elif name == "pv2_topk_distill_forward":
+        x, _, m, v, ldx, index, is64, ldi, t, _, ldt, k, temperature, mean, _, _, row_loss, loss, count = args
+        ids = np.lib.stride_tricks.as_strided(ids_at(index, is64, (m - 1) * ldi + k), (m, k),
+                                              (ldi * (8 if is64 else 4), 8 if is64 else 4))
+        rows, _, counts, *_ = distill(*(torch.from_numpy(a.copy()) for a in (
+            matrix_at(x, m, v, ldx), ids, matrix_at(t, m, k, ldt))), temperature)
+        at(count, 1, ctypes.c_float)[0] = counts.sum()
+        at(loss, 1, ctypes.c_float)[0] = rows.sum() / max(1, counts.sum()) if mean else rows.sum()
+        if row_loss is not None:
+            at(row_loss, m, ctypes.c_float)[:] = rows
     else:
         raise AssertionError(name)
 
@@ -64,7 +78,7 @@ def statement(name, device, *args):
 def where(request, monkeypatch):
     if request.param == "device":
         return request.getfixturevalue("device")
-    for module in (row_groups, embedding_module, grouped_linear_module):
+    for module in (row_groups, embedding_module, grouped_linear_module, distillation_module):
         monkeypatch.setattr(module, "launch", statement)
         monkeypatch.setattr(module, "_require_device", lambda *tensors: None)
     return torch.device("cpu")
@@ -192,3 +206,39 @@ def test_traced_groups_replay(where):
         y, offsets = traced(x, w, torch.tensor(counts[:3], device=where).cumsum(0))
         assert offsets.tolist() == [0, *np.cumsum(counts[:3])]
         assert torch.equal(y, products(x, w, index, torch.zeros_like(b)))
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_a_traced_distillation_replays(where, reduction):
+    def lists(shape, v, k):
+        return (torch.randn(*shape, v, device=where), torch.randint(-1, v, (*shape, k), device=where),
+                torch.randn(*shape, k, device=where))
+
+    def check(logits, index, teacher):
+        fill_free_memory(where)
+        rows, _, counts, big, *_ = distill(logits.reshape(-1, logits.shape[-1]), index.reshape(-1, index.shape[-1]),
+                                           teacher.reshape(-1, teacher.shape[-1]), 2.0)
+        want = rows.reshape(logits.shape[:-1]) if reduction == "none" else rows.sum() / counts.sum().clamp(min=1)
+        got = traced(logits, index, teacher)
+        assert got.shape == want.shape and got.dtype == torch.float32
+        # as tests/test_gpu_distillation.py: T^2 (8 |log| + V / 64 + 32) (2 + 2 |log|) roundings of a row; 64 for the mean's sum
+        unit = 4 * (8 * big.max() + logits.shape[-1] / 64 + 32) * (2 + 2 * big.max()) * EPS32
+        assert float((got.double() - want).abs().max()) <= float(unit + 64 * EPS32 * rows.abs().max())
+
+    args = lists((20,), 9, 3)
+    traced = trace(lambda s, i, t: topk_distillation(s, i, t, 2.0, reduction), *args)
+    check(*args)
+    for shape, v, k in (((31,), 9, 3), ((1,), 600, 5), ((4, 5), 12, 2)):
+        logits, index, teacher = lists(shape, v, k)
+        check(logits, index, teacher)
+        check(logits, index.int(), teacher)
+        check(logits.transpose(0, -1).contiguous().transpose(0, -1), index, teacher)
+        check(torch.randn(*shape, v + 7, device=where)[..., 3:3 + v], index, teacher)
+    for bad in ((logits, index.float(), teacher), (logits, index[:2], teacher[:2]), (logits.double(), index, teacher),
+                (logits, index[..., :1], teacher)):
+        with pytest.raises(Exception, match="topk_distillation: "):
+            traced(*bad)
+    empty = traced(torch.zeros(0, 9, device=where), torch.zeros(0, 3, dtype=torch.int64, device=where),
+                   torch.zeros(0, 3, device=where))
+    assert empty.shape == ((0,) if reduction == "none" else ()) and not empty.any()
