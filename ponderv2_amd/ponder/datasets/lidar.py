@@ -14,9 +14,9 @@ The produced sample follows the ``Collect`` of configs/nuscenes/pretrain-ponder-
 import numpy as np
 import torch
 
-from .voxelize import GridSample
+from .voxelize import TEACHER_ARRAYS, GridSample
 
-POINT_KEYS = ("color", "normal", "strength", "segment", "instance")
+POINT_KEYS = ("color", "normal", "strength", "segment", "instance") + TEACHER_ARRAYS
 
 
 class PointRangeFilter:

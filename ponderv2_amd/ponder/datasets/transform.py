@@ -24,13 +24,13 @@ import torch
 
 from ..utils.registry import Registry
 from .lidar import PointRangeFilter, ProjectOnImage, RaySample
-from .voxelize import GridSample
+from .voxelize import TEACHER_ARRAYS, GridSample
 
 TRANSFORMS = Registry("transforms")
 for _cls in (GridSample, PointRangeFilter, ProjectOnImage, RaySample):
     TRANSFORMS.register_module(module=_cls, name=_cls.__name__)
 
-POINT_ARRAYS = ("coord", "color", "normal", "strength", "segment", "instance")
+POINT_ARRAYS = ("coord", "color", "normal", "strength", "segment", "instance") + TEACHER_ARRAYS
 
 
 def _follow_cameras(data_dict, keys, S):
@@ -278,7 +278,7 @@ class ShufflePoint:
         order = np.arange(data_dict["coord"].shape[0])
         np.random.shuffle(order)
         _select_rows(data_dict, order, ("coord", "grid_coord", "displacement", "color", "normal",
-                                        "segment", "instance"))
+                                        "segment", "instance") + TEACHER_ARRAYS)
         return data_dict
 
 

@@ -9,6 +9,10 @@ import os
 
 import numpy as np
 
+# a teacher's lists of a point (models/losses: TopLogitsDistillLoss), (N, k) each: whatever selects or reorders points takes
+# them along where a sample has them
+TEACHER_ARRAYS = ("teacher_index", "teacher_logits")
+
 _FNV_OFFSET = np.uint64(14695981039346656037)
 _FNV_PRIME = np.uint64(1099511628211)
 
@@ -65,7 +69,7 @@ class GridSample:
             data_dict["grid_coord"] = grid_coord[idx_unique]
         if self.return_min_coord:
             data_dict["min_coord"] = min_coord.reshape([1, 3])
-        for k in self.keys:
+        for k in (*self.keys, *(t for t in TEACHER_ARRAYS if t in data_dict and t not in self.keys)):
             data_dict[k] = data_dict[k][idx_unique]
         return data_dict
 
@@ -243,14 +247,14 @@ def device_grid_sample(batch, grid_size=0.02, hash_type="fnv", keys=("coord", "f
     """Train-mode GridSample of a collated batch of RAW points on whatever device the batch lives
     on (the GPU, after the trainer's host->device copy): per scene - the rows between consecutive
     ``offset`` entries - one representative per occupied voxel, in the host transform's voxel order
-    (``grid_sample_torch``).  Rewrites ``keys`` and ``offset`` and adds ``grid_coord``; every other
-    entry (images, poses, ...) passes through.  This is the device half of SURVEY 8(f) F3: the
+    (``grid_sample_torch``).  Rewrites ``keys``, a teacher's lists and ``offset`` and adds
+    ``grid_coord``; every other entry (images, poses, ...) passes through.  This is the device half of SURVEY 8(f) F3: the
     loader workers then only stream raw points (``voxelize=False`` on the synthetic datasets).
     ``picks``: optional list of per-scene tensors standing in for the transform's random draws."""
     import torch
 
     ends = batch.get("offset_host") or batch["offset"].tolist()   # one read of B small numbers
-    out = {k: [] for k in keys if k in batch}
+    out = {k: [] for k in (*keys, *TEACHER_ARRAYS) if k in batch}
     grids, new_ends, start = [], [], 0
     for b, end in enumerate(ends):
         # device tensors: the HIP hash-insert / segmented-pick kernels (csrc/voxelize.hip); host
