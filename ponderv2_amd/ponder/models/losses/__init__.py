@@ -71,7 +71,15 @@ class Criteria:
         """``teacher``: (index, logits) of the criteria that are taken against a teacher's lists."""
         if not self.criteria:
             return pred  # loss computed inside the model
-        return sum(c(pred, teacher if getattr(c, "from_teacher", False) else target) for c in self.criteria)
+        return sum(c(pred, self._lists(c, teacher) if getattr(c, "from_teacher", False) else target)
+                   for c in self.criteria)
+
+    @staticmethod
+    def _lists(criterion, teacher):
+        if teacher is None:
+            raise ValueError(f"{type(criterion).__name__}: the batch carries no teacher's lists (teacher_index and "
+                             "teacher_logits, one row per point; Collect names both)")
+        return teacher
 
 
 def build_criteria(cfg):

@@ -492,7 +492,8 @@ class PonderIndoor(nn.Module):
         sim = linear(feat, self._valid_embedding(self._condition_index(data_dict), feat.device))
         # a criterion that is taken against a teacher (losses.TopLogitsDistillLoss) finds its lists, class numbers of
         # this condition's valid classes, in the batch
-        teacher = ((data_dict["teacher_index"], data_dict["teacher_logits"]) if "teacher_index" in data_dict else None)
+        teacher = tuple(data_dict[k] for k in ("teacher_index", "teacher_logits") if k in data_dict)
+        teacher = teacher if len(teacher) == 2 else None
         return self.ppt_criteria(self.logit_scale.exp() * sim, data_dict["segment"], teacher)
 
     def _projection_dtype(self, device):

@@ -7,6 +7,9 @@ import torch
 from ponderv2_amd.ponder.datasets.collate import point_collate_fn
 from ponderv2_amd.ponder.datasets.transform import Compose
 from ponderv2_amd.ponder.datasets.voxelize import device_grid_sample
+from ponderv2_amd.ponder.models.losses import build_criteria
+from ponderv2_amd.ponder.models.ponder.ponder_indoor_base import PonderIndoor
+from test_distill_loss import ppt
 
 N, K = 3000, 4
 
@@ -91,3 +94,15 @@ def test_samples_without_lists_are_as_before():
         assert "teacher_index" not in b
         for k in b:
             assert np.array_equal(a[k], b[k]), k
+
+
+@pytest.mark.parametrize("missing", [("teacher_index", "teacher_logits"), ("teacher_logits",), ("teacher_index",)])
+def test_a_batch_without_lists_is_refused_by_name(missing):
+    """As a dataset without a teacher among others brings it; the other criteria do not ask for lists."""
+    model, batch = ppt(torch.device("cpu"))
+    for key in missing:
+        del batch[key]
+    with pytest.raises(ValueError, match="TopLogitsDistillLoss: the batch carries no teacher's lists"):
+        PonderIndoor.ppt_loss(model, batch)
+    model.ppt_criteria = build_criteria([dict(type="CrossEntropyLoss", loss_weight=1.0, ignore_index=-1)])
+    assert torch.isfinite(PonderIndoor.ppt_loss(model, batch))
