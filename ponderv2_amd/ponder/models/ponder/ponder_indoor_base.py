@@ -493,8 +493,8 @@ class PonderIndoor(nn.Module):
         # a criterion that is taken against a teacher (losses.TopLogitsDistillLoss) finds its lists, class numbers of
         # this condition's valid classes, in the batch
         teacher = tuple(data_dict[k] for k in ("teacher_index", "teacher_logits") if k in data_dict)
-        teacher = teacher if len(teacher) == 2 else None
-        return self.ppt_criteria(self.logit_scale.exp() * sim, data_dict["segment"], teacher)
+        more = dict(teacher=teacher) if len(teacher) == 2 else {}   # (criteria of two arguments are called with two)
+        return self.ppt_criteria(self.logit_scale.exp() * sim, data_dict["segment"], **more)
 
     def _projection_dtype(self, device):
         """Reduced precision of the dense projection network: ``proj_autocast`` (a dtype name) or

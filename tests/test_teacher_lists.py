@@ -106,3 +106,11 @@ def test_a_batch_without_lists_is_refused_by_name(missing):
         PonderIndoor.ppt_loss(model, batch)
     model.ppt_criteria = build_criteria([dict(type="CrossEntropyLoss", loss_weight=1.0, ignore_index=-1)])
     assert torch.isfinite(PonderIndoor.ppt_loss(model, batch))
+
+
+def test_criteria_of_two_arguments():
+    """A model whose criteria are a callable (pred, target) of its own is called with two, as ever."""
+    model, batch = ppt(torch.device("cpu"))
+    del batch["teacher_index"], batch["teacher_logits"]
+    model.ppt_criteria = lambda pred, target: torch.nn.functional.cross_entropy(pred, target, ignore_index=-1)
+    assert torch.isfinite(PonderIndoor.ppt_loss(model, batch))
