@@ -16,6 +16,7 @@
 // launches; 1 000 003 ids over 50 021 groups 57 us (count 6.5, scan 4.4, scatter 14.4 per pass, offsets 7; 12.2 MB at the rate
 // of a copy are 2.4).
 #include "common.h"
+#include "sorted_search.h"
 
 namespace {
 
@@ -226,21 +227,11 @@ __global__ __launch_bounds__(kThreads) void scatter_kernel(Source src, const int
   }
 }
 
-// first position of a sorted key >= v
-__device__ __forceinline__ int lower_bound(const int32_t* keys, int n, int v) {
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (keys[mid] < v) lo = mid + 1; else hi = mid;
-  }
-  return lo;
-}
-
 __global__ __launch_bounds__(kThreads) void offsets_kernel(const int32_t* __restrict__ keys, int64_t n, int n_groups,
                                                            int32_t* __restrict__ offsets) {
   const int64_t stride = (int64_t)gridDim.x * kThreads;
   for (int64_t g = (int64_t)blockIdx.x * kThreads + threadIdx.x; g <= n_groups; g += stride)
-    offsets[g] = lower_bound(keys, (int)n, (int)g);
+    offsets[g] = pv2::lower_bound(keys, (int)n, (int)g);
 }
 
 // All passes of at most kSmall keys in one workgroup; every wave owns a contiguous share of the positions.
@@ -301,7 +292,7 @@ __global__ __launch_bounds__(kSmallThreads) void small_kernel(Source src, int n,
     if (keys_out) keys_out[i] = s_key[cur][i];
   }
   if (offsets)
-    for (int g = tid; g <= n_groups; g += kSmallThreads) offsets[g] = lower_bound(s_key[cur], n, g);
+    for (int g = tid; g <= n_groups; g += kSmallThreads) offsets[g] = pv2::lower_bound(s_key[cur], n, g);
 }
 
 // cumulative row counts (B,) -> offsets [B + 1], never decreasing and within 0 .. n whatever the counts hold
