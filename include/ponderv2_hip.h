@@ -1063,7 +1063,7 @@ int pv2_row_offsets(const void* cumulative, int is_64, int64_t n_groups, int64_t
  * `row_stride` elements between rows; out is contiguous and of the weight's type (PV2_F32 / PV2_BF16 / PV2_F16).
  * Backward: grad_weight [rows, c] (contiguous, every element written, of the same type) = scale * the sum of the rows
  * of grad_out whose index it is, in a fixed order, in fp32, rounded once.  workspace: 32-byte aligned,
- * pv2_embedding_backward_workspace_ints(n, rows, c) ints. */
+ * pv2_embedding_backward_workspace_ints(n, rows, c) ints.  c < 2^30. */
 int pv2_embedding_forward(const void* index, int index_is_64, int64_t n, const void* weight, int dtype, int64_t rows,
                           int c, int64_t row_stride, float scale, void* out, pv2_stream_t stream);
 int64_t pv2_embedding_backward_workspace_ints(int64_t n, int64_t rows, int c);

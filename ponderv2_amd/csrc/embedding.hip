@@ -24,6 +24,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kPiece = 32;
 constexpr int kBlock = 32 * kPiece;
+constexpr int kMaxWidth = 1 << 30;   // columns and what a workgroup adds to them stay below 2^31
 
 struct F32 {
   typedef float type;
@@ -370,7 +371,7 @@ extern "C" {
 int pv2_embedding_forward(const void* index, int index_is_64, int64_t n, const void* weight, int dtype, int64_t rows,
                           int c, int64_t row_stride, float scale, void* out, pv2_stream_t stream) {
   PV2_REQUIRE(index && weight && out, "embedding_forward: null pointer");
-  PV2_REQUIRE(n > 0 && rows > 0 && c > 0 && row_stride >= 0, "embedding_forward: bad shape");
+  PV2_REQUIRE(n > 0 && rows > 0 && c > 0 && c < kMaxWidth && row_stride >= 0, "embedding_forward: bad shape");
   hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
     case PV2_F32: return forward<F32>(index, index_is_64, n, weight, rows, c, row_stride, scale, out, s);
@@ -388,7 +389,7 @@ int pv2_embedding_backward(const void* index, int index_is_64, int64_t n, const 
                            int c, int64_t grad_row_stride, float scale, int32_t* workspace, void* grad_weight,
                            pv2_stream_t stream) {
   PV2_REQUIRE(grad_weight && workspace && (n == 0 || (index && grad_out)), "embedding_backward: null pointer");
-  PV2_REQUIRE(n >= 0 && rows > 0 && c > 0 && grad_row_stride >= 0, "embedding_backward: bad shape");
+  PV2_REQUIRE(n >= 0 && rows > 0 && c > 0 && c < kMaxWidth && grad_row_stride >= 0, "embedding_backward: bad shape");
   PV2_REQUIRE((uintptr_t)workspace % 32 == 0, "embedding_backward: workspace not aligned to 32 bytes");
   hipStream_t s = (hipStream_t)stream;
   const Layout l = layout_of(n, rows, c);

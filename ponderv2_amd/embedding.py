@@ -11,6 +11,8 @@ from .kernels import DTYPE_CODE, _require_device
 from .row_groups import (MAX_GROUPS, MAX_ROWS, launch, launch_alone, once_differentiable_backward, ptr,
                          require_index)
 
+MAX_WIDTH = (1 << 30) - 1
+
 
 def _checked(index, weight):
     """The ids as one list and the table with contiguous rows.  Part of every pass through the operator, so that a replayed
@@ -18,13 +20,13 @@ def _checked(index, weight):
     require_index(index, "embedding")
     if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError(f"embedding: weight is (rows, channels), got {tuple(weight.shape)}")
+    if index.numel() > MAX_ROWS or weight.shape[0] > MAX_GROUPS or weight.shape[1] > MAX_WIDTH:
+        raise ValueError(f"embedding: up to {MAX_ROWS} indices, {MAX_GROUPS} rows and {MAX_WIDTH} channels")
     if weight.dtype not in DTYPE_CODE:
         raise TypeError(f"embedding: float32, bfloat16 or float16 weight expected, got {weight.dtype}")
     _require_device(index, weight)
     if index.device != weight.device:
         raise ValueError(f"embedding: index on {index.device}, weight on {weight.device}")
-    if index.numel() > MAX_ROWS or weight.shape[0] > MAX_GROUPS:
-        raise ValueError(f"embedding: up to {MAX_ROWS} indices and {MAX_GROUPS} rows")
     flat = index if index.dim() == 1 and index.is_contiguous() else index.reshape(-1).contiguous()
     return flat, rows_contiguous(weight)
 
