@@ -194,7 +194,7 @@ struct Item {
   int group;       // n_groups: the rows of no group; -1: no such item
   int first, last; // positions
   int number, of;  // which of the group's items this is
-  int base;        // the group's first item
+  int slab;        // of the items of groups that have more than one: which this is
 };
 
 // The item of workgroup `id` when every group's rows are cut into pieces of `unit` (`empty`: a group without rows has one
@@ -203,7 +203,7 @@ struct Item {
 // and an item's rows are read into one L2 only (items dealt in turn instead: 124 -> 100 us for 32768 rows, 16 groups,
 // 1024 x 1024, bf16).
 __device__ __forceinline__ Item find_item(const int32_t* __restrict__ offsets, int n_groups, int n_rows, int unit,
-                                          bool empty, int id, int tiles, int* item_out, int* tile) {
+                                          bool empty, int id, int tiles, int* tile) {
   const int lane = threadIdx.x & 63;
   int from = 0, to = 0, count = 0, upto = 0;
   auto scan = [&](int g0) {   // counts of groups g0 .. g0 + 63 and their prefix sums
@@ -228,18 +228,17 @@ __device__ __forceinline__ Item find_item(const int32_t* __restrict__ offsets, i
   const int per_xcd = (total + 7) / 8, k = id / 8 / tiles;
   const int item = id % 8 * per_xcd + k;
   *tile = id / 8 % tiles;
-  *item_out = item;
   Item it = {-1, 0, 0, 0, 0, 0};
   if (k >= per_xcd || item >= total) return it;
-  int run = 0;
+  int run = 0, single = 0;   // items of the groups before; how many of those groups have one item only
   for (int g0 = 0; g0 <= n_groups; g0 += 64) {
     const int sum = n_groups < 64 ? total : scan(g0);   // (one round: it is there already)
-    const uint64_t past = __ballot(run + upto > item);
+    const uint64_t past = __ballot(run + upto > item), ones = __ballot(count == 1);
     if (past) {
       const int l = __ffsll((unsigned long long)past) - 1;
       it.of = __shfl(count, l);
-      it.base = run + __shfl(upto, l) - it.of;
-      it.number = item - it.base;
+      it.number = item - (run + __shfl(upto, l) - it.of);
+      it.slab = item - single - __popcll(ones & ((1ull << l) - 1));
       it.group = g0 + l;
       const int f = __shfl(from, l), t = __shfl(to, l);
       // (a group's items of a weight gradient are about equal: whole steps of 32 rows, the last one may be empty)
@@ -249,6 +248,7 @@ __device__ __forceinline__ Item find_item(const int32_t* __restrict__ offsets, i
       return it;
     }
     run += sum;
+    single += __popcll(ones);
   }
   return it;
 }
@@ -307,8 +307,8 @@ __global__ __launch_bounds__(kThreads, 3) void rows_kernel(
   u16 *s_w = s_all, *s_x = s_all + PL * kPlane;
   __shared__ int s_row[kTile];
   __shared__ __attribute__((aligned(16))) float s_bias[kTile];
-  int item, tile;
-  const Item it = find_item(offsets, n_groups, n_rows, kTile, false, blockIdx.x, n_tiles, &item, &tile);
+  int tile;
+  const Item it = find_item(offsets, n_groups, n_rows, kTile, false, blockIdx.x, n_tiles, &tile);
   if (it.group < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int c0 = tile * kTile;
@@ -429,8 +429,8 @@ __global__ __launch_bounds__(kThreads, 3) void wgrad_kernel(
   constexpr int D = P::kDepth, PL = P::kPlanes, kPlane = kTile * D, U = kChunks<P>;
   __shared__ __attribute__((aligned(16))) u16 s_all[kLds<P>];
   u16 *s_x = s_all, *s_g = s_all + PL * kPlane;
-  int item, tile;
-  const Item it = find_item(offsets, n_groups, n_rows, unit, true, blockIdx.x, tiles_out * tiles_in, &item, &tile);
+  int tile;
+  const Item it = find_item(offsets, n_groups, n_rows, unit, true, blockIdx.x, tiles_out * tiles_in, &tile);
   if (it.group < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int n0 = tile / tiles_in * kTile, k0 = tile % tiles_in * kTile;
@@ -532,7 +532,7 @@ __global__ __launch_bounds__(kThreads, 3) void wgrad_kernel(
   };
   const int64_t size = (int64_t)n_out * n_in;
   if (whole) leave(reinterpret_cast<E*>(s_all), dw + it.group * size);
-  else leave(reinterpret_cast<float*>(s_all), dw_part + item * size);
+  else leave(reinterpret_cast<float*>(s_all), dw_part + it.slab * size);
   if (sum_bias) {
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -540,7 +540,7 @@ __global__ __launch_bounds__(kThreads, 3) void wgrad_kernel(
       const int n = n0 + wn * 64 + b * 32 + i;
       if (h != 0 || n >= n_out) continue;
       if (whole) db[(int64_t)it.group * n_out + n] = P::from_float(sum);
-      else db_part[(int64_t)item * n_out + n] = sum;
+      else db_part[(int64_t)it.slab * n_out + n] = sum;
     }
   }
 }
@@ -660,8 +660,8 @@ __global__ __launch_bounds__(2 * ROWS, 2) void rows_direct_kernel(
   __shared__ __attribute__((aligned(1024))) u16 s_all[2 * kBuffer > kOut ? 2 * kBuffer : kOut];   // (addresses are XORed)
   __shared__ int s_row[ROWS];
   __shared__ __attribute__((aligned(16))) float s_bias[COLS];
-  int item, tile;
-  const Item it = find_item(offsets, n_groups, n_rows, ROWS, false, blockIdx.x, n_tiles, &item, &tile);
+  int tile;
+  const Item it = find_item(offsets, n_groups, n_rows, ROWS, false, blockIdx.x, n_tiles, &tile);
   if (it.group < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c0 = tile * COLS;
@@ -810,8 +810,8 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_direct_kernel(
   constexpr int kOut = 64 * kOutRow<float, COLS> * 2;
   __shared__ __attribute__((aligned(16))) u16 s_all[kBuffers * kBuffer > kOut ? kBuffers * kBuffer : kOut];
   __shared__ int s_row[kSegment];
-  int item, tile;
-  const Item it = find_item(offsets, n_groups, n_rows, unit, true, blockIdx.x, tiles_out * tiles_in, &item, &tile);
+  int tile;
+  const Item it = find_item(offsets, n_groups, n_rows, unit, true, blockIdx.x, tiles_out * tiles_in, &tile);
   if (it.group < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n0 = tile / tiles_in * kTile, k0 = tile % tiles_in * COLS;
@@ -946,7 +946,7 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_direct_kernel(
   };
   const int64_t size = (int64_t)n_out * n_in;
   if (whole) leave(s_all, dw + it.group * size);
-  else leave(reinterpret_cast<float*>(s_all), dw_part + item * size);
+  else leave(reinterpret_cast<float*>(s_all), dw_part + it.slab * size);
   if (sum_bias) {
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -954,7 +954,7 @@ __global__ __launch_bounds__(kThreads, 2) void wgrad_direct_kernel(
       const int n = n0 + wn * 64 + b * 32 + i;
       if (h != 0 || n >= n_out) continue;
       if (whole) db[(int64_t)it.group * n_out + n] = H::from_float(sum);
-      else db_part[(int64_t)item * n_out + n] = sum;
+      else db_part[(int64_t)it.slab * n_out + n] = sum;
     }
   }
 }
@@ -973,10 +973,13 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const int32_t* __restric
   const int from = offsets[g], to = offsets[g + 1];
   const int count = (to - from + unit - 1) / unit;
   if (count <= 1) return;
-  // the group's first item: all items of the groups before it
+  // the group's first partial result: all items of the groups before it that have more than one
   __shared__ int s_base[kThreads / 64];
   int base = 0;
-  for (int f = threadIdx.x; f < g; f += kThreads) base += max(1, (offsets[f + 1] - offsets[f] + unit - 1) / unit);
+  for (int f = threadIdx.x; f < g; f += kThreads) {
+    const int items = (offsets[f + 1] - offsets[f] + unit - 1) / unit;
+    base += items > 1 ? items : 0;
+  }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) base += __shfl_xor(base, d);
   if ((threadIdx.x & 63) == 0) s_base[threadIdx.x >> 6] = base;
@@ -1038,8 +1041,8 @@ __global__ __launch_bounds__(kThreads) void few_rows_kernel(
   typedef Few<P> F;
   constexpr int U = 4;
   __shared__ f32x4 s_part[kThreads / 64][64];
-  int item, tile;
-  const Item it = find_item(offsets, n_groups, n_rows, 16, false, blockIdx.x, n_tiles, &item, &tile);
+  int tile;
+  const Item it = find_item(offsets, n_groups, n_rows, 16, false, blockIdx.x, n_tiles, &tile);
   if (it.group < 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i = lane & 15, h = lane >> 4;
@@ -1156,7 +1159,7 @@ int launch_rows(const void* x, int64_t ldx, const void* w, int64_t w_group, int6
 
 struct Split {   // of the weight gradient
   int unit;
-  int64_t items;
+  int64_t items, slabs;   // most items; most of them that leave a partial result: those of groups of more than `unit` rows
 };
 
 // Writing and reading an item's partial result costs as much as the products of some 700 rows (16-bit) or 150 (fp32), and
@@ -1170,7 +1173,10 @@ Split split_of(int dtype, int64_t rows, int64_t groups, int n_out, int n_in) {
   const int64_t least = full ? 256 : 1024;
   if (unit < least) unit = least;
   unit = (unit + 63) / 64 * 64;
-  return {(int)unit, rows / unit + groups};
+  // a group of r rows has c = 1 + (r - 1) / unit items: the (r - 1) / unit of all groups add up to `more` at most, and no
+  // more groups than that have two items or more
+  const int64_t more = rows > 0 ? (rows - 1) / unit : 0;
+  return {(int)unit, rows / unit + groups, more + (more < groups ? more : groups)};
 }
 
 template <class P>
@@ -1187,7 +1193,7 @@ int launch_wgrad(const void* dy, int64_t ldy, const void* x, int64_t ldx, const 
   const int64_t size = (int64_t)n_out * n_in;
   const bool parts = rows > sp.unit;
   PV2_REQUIRE(!parts || ws, "grouped_linear: no workspace");
-  float* db_part = parts ? ws + sp.items * size : nullptr;
+  float* db_part = parts ? ws + sp.slabs * size : nullptr;
 #define PV2_WGRAD(kernel)                                                                                            \
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), 0, s, (const E*)dy, ldy, (const E*)x, ldx, order, \
                      offsets, (int)rows, (int)groups, n_out, n_in, sp.unit, to, ti, (E*)dw, (E*)db, ws, db_part)
@@ -1256,7 +1262,7 @@ int pv2_grouped_linear_grad_input(const void* grad_out, int dtype, int64_t rows,
 int64_t pv2_grouped_linear_workspace_floats(int dtype, int64_t rows, int64_t groups, int n_out, int n_in) {
   if (rows < 1 || groups < 1 || n_out < 1 || n_in < 1) return 0;
   const Split sp = split_of(dtype, rows, groups, n_out, n_in);
-  return rows > sp.unit ? sp.items * ((int64_t)n_out * n_in + n_out) : 0;
+  return sp.slabs * ((int64_t)n_out * n_in + n_out);
 }
 
 int pv2_grouped_linear_grad_weight(const void* grad_out, int dtype, int64_t rows, int n_out, int64_t grad_stride,

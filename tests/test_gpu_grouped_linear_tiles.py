@@ -1,0 +1,64 @@
+"""grouped_linear() on whole numbers so small that every product and every sum is exact in fp32: results have to equal the
+64-bit ones after one rounding, whatever the number of rows, so that a row left out or taken twice shows."""
+import pytest
+import torch
+
+from ponderv2_amd.grouped_linear import grouped_linear
+from ponderv2_amd.row_groups import group_rows
+from row_ops_oracle import DTYPES
+
+pytestmark = pytest.mark.gpu
+
+
+def whole(low, high, *shape, device, dtype):
+    return torch.randint(low, high + 1, shape, device=device).to(dtype)
+
+
+def products(x, w, index, bias, gy):
+    """The definition in fp32 where it is exact: sums of whole numbers below 2^24 (by torch, group by group)."""
+    x, w, bias, gy = (t.float() for t in (x, w, bias, gy))
+    y, d_x, d_w, d_b = x.new_zeros(len(x), w.shape[1]), torch.zeros_like(x), torch.zeros_like(w), torch.zeros_like(bias)
+    for e in range(len(w)):
+        r = torch.nonzero(index == e)[:, 0]
+        y[r], d_x[r] = x[r] @ w[e].T + bias[e], gy[r] @ w[e]
+        d_w[e], d_b[e] = gy[r].T @ x[r], gy[r].sum(0)
+    return y, d_x, d_w, d_b
+
+
+def check(m, sizes, k, n, dtype, device, most=2):
+    """Groups of ``sizes`` rows (the rest of the m rows in no group), in random order."""
+    g = len(sizes)
+    index = torch.cat([torch.repeat_interleave(torch.arange(g), torch.tensor(sizes)),
+                       torch.full((m - sum(sizes),), -1)])[torch.randperm(m)].to(device)
+    x, w = whole(-most, most, m, k, device=device, dtype=dtype), whole(-most, most, g, n, k, device=device, dtype=dtype)
+    bias, gy = whole(-9, 9, g, n, device=device, dtype=dtype), whole(-1, 1, m, n, device=device, dtype=dtype)
+    assert max(most * most * k + 9, most * n, most * max(sizes)) < 2 ** 24
+    leaves = [t.detach().requires_grad_() for t in (x, w, bias)]
+    y = grouped_linear(leaves[0], leaves[1], group_rows(index, g), leaves[2])
+    grads = torch.autograd.grad(y, leaves, gy)
+    for name, got, want in zip(("y", "d_x", "d_w", "d_b"), (y.detach(), *grads), products(x, w, index, bias, gy)):
+        assert torch.equal(got, want.to(dtype)), f"{name}: {int((got != want.to(dtype)).sum())} values differ"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k,n", [(40, 24), (33, 17)])
+def test_split_groups_among_many(dtype, k, n, device):
+    """Groups of no, one, two and many pieces next to each other, in every 64 of more than 200."""
+    torch.manual_seed(20)
+    sizes = [(0, 1, 5, 256, 257, 1024, 1025, 300, 3000, 513, 0, 2049, 64)[i % 13] for i in range(201)]
+    check(sum(sizes) + 77, sizes, k, n, dtype, device)
+
+
+def test_memory_of_a_weight_gradient_with_many_groups(device):
+    """4096 groups of 256 x 256: beside the gradient (0.5 GB in bf16) partial results of a few split groups only."""
+    torch.manual_seed(21)
+    m, g, k = 20000, 4096, 256
+    x, gy = (whole(-2, 2, m, k, device=device, dtype=torch.bfloat16) for _ in range(2))
+    w = torch.zeros(g, k, k, device=device, dtype=torch.bfloat16, requires_grad=True)
+    groups = group_rows(torch.randint(0, g, (m,), device=device), g)
+    y = grouped_linear(x, w, groups)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    torch.autograd.grad(y, w, gy)
+    assert torch.cuda.max_memory_allocated() - before <= 1.1 * w.numel() * 2

@@ -22,3 +22,18 @@ def test_embedding_width_of_the_entries():
     L, p, n = _lib.lib(), ctypes.c_void_p(64), None
     assert L.pv2_embedding_forward(p, 1, 4, p, 0, 3, 1 << 30, 1 << 30, 1.0, p, n) == BADARG
     assert L.pv2_embedding_backward(p, 1, 4, p, 0, 3, 1 << 30, 1 << 30, 1.0, p, p, n) == BADARG
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_workspace_of_a_weight_gradient_does_not_grow_with_the_groups(dtype):
+    """Only groups that are split leave partial results: 32768 rows have at most 2 * 32767 / 256 of them (16-bit types take
+    pieces of 1024 rows or more), however many groups there are."""
+    L = _lib.lib()
+    slab = 512 * 512 + 512
+    floats = [L.pv2_grouped_linear_workspace_floats(dtype, 32768, g, 512, 512) for g in (1, 64, 512, 4096)]
+    most = 2 * (32767 // (256 if dtype == 0 else 1024)) * slab
+    assert 0 < floats[0] <= most and all(f <= most for f in floats)
+    # 20000 rows over 4096 groups: no more than 38 slabs beside a gradient of 4096
+    assert L.pv2_grouped_linear_workspace_floats(1, 20000, 4096, 1024, 1024) <= 38 * (1024 * 1024 + 1024)
+    for rows in (1, 255, 256):   # none can be split
+        assert L.pv2_grouped_linear_workspace_floats(dtype, rows, 8, 64, 64) == 0
