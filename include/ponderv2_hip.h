@@ -1079,6 +1079,8 @@ int pv2_embedding_backward(const void* index, int index_is_64, int64_t n, const 
  *                rows of no group are zeros in both
  *   grad_weight  grad_weight [groups, n_out, n_in] = grad_out_g^T x_g, grad_bias [groups, n_out] = sum of grad_out_g;
  *                every element written; workspace: pv2_grouped_linear_workspace_floats (may be null if that is 0).
+ *                grad_weight null: grad_bias alone, x is not read (may be null), workspace:
+ *                pv2_grouped_linear_bias_workspace_floats of the same sizes.
  * At most 4096 groups; rows < 2^30.  order and offsets are not checked. */
 int pv2_grouped_linear_forward(const void* x, int dtype, int64_t rows, int n_in, int64_t x_stride, const void* weight,
                                int64_t weight_group_stride, int64_t weight_row_stride, int64_t groups, int n_out,
@@ -1089,10 +1091,11 @@ int pv2_grouped_linear_grad_input(const void* grad_out, int dtype, int64_t rows,
                                   int64_t groups, int n_in, const int32_t* order_or_null, const int32_t* offsets,
                                   void* grad_x, pv2_stream_t stream);
 int64_t pv2_grouped_linear_workspace_floats(int dtype, int64_t rows, int64_t groups, int n_out, int n_in);
+int64_t pv2_grouped_linear_bias_workspace_floats(int dtype, int64_t rows, int64_t groups, int n_out, int n_in);
 int pv2_grouped_linear_grad_weight(const void* grad_out, int dtype, int64_t rows, int n_out, int64_t grad_stride,
                                    const void* x, int n_in, int64_t x_stride, int64_t groups,
                                    const int32_t* order_or_null, const int32_t* offsets, float* workspace,
-                                   void* grad_weight, void* grad_bias_or_null, pv2_stream_t stream);
+                                   void* grad_weight_or_null, void* grad_bias_or_null, pv2_stream_t stream);
 
 /* ---- Distillation from a teacher's top logits (csrc/distillation.hip) -------------------------------------------
  * Row i: p = softmax(teacher_logits[i] / T) over its listed classes (teacher_index[i], k of them; an entry counts if its

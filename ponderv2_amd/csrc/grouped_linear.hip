@@ -419,7 +419,8 @@ __global__ __launch_bounds__(kThreads, 3) void rows_kernel(
 }
 
 // dW[g][n][k] over one item's rows.  The item is the whole group: written in the weights' type; else fp32 partials.
-template <class P>
+// WEIGHTS false: db alone, the same sums in the same order; x is not read (tiles_in is 1).
+template <class P, bool WEIGHTS>
 __global__ __launch_bounds__(kThreads, 3) void wgrad_kernel(
     const typename P::E* __restrict__ dy, int64_t ldy, const typename P::E* __restrict__ x, int64_t ldx,
     const int32_t* __restrict__ order, const int32_t* __restrict__ offsets, int n_rows, int n_groups, int n_out,
@@ -454,7 +455,7 @@ __global__ __launch_bounds__(kThreads, 3) void wgrad_kernel(
       const int q = tid + u * kThreads, row = q / (kTile / 8);
       const int col = ((q % (kTile / 8)) ^ across_swizzle(row)) * 8;
       const int64_t r = row_of[u];
-      rx[u] = r >= 0 && k0 + col < n_in ? P::load(x + r * ldx + k0 + col, n_in - k0 - col) : P::zero();
+      if (WEIGHTS) rx[u] = r >= 0 && k0 + col < n_in ? P::load(x + r * ldx + k0 + col, n_in - k0 - col) : P::zero();
       rg[u] = r >= 0 && n0 + col < n_out ? P::load(dy + r * ldy + n0 + col, n_out - n0 - col) : P::zero();
     }
   };
@@ -474,7 +475,7 @@ __global__ __launch_bounds__(kThreads, 3) void wgrad_kernel(
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int q = tid + u * kThreads;
-      P::stage(s_x + q * 8, kPlane, rx[u]);
+      if (WEIGHTS) P::stage(s_x + q * 8, kPlane, rx[u]);
       P::stage(s_g + q * 8, kPlane, rg[u]);
     }
     __syncthreads();
@@ -491,7 +492,7 @@ __global__ __launch_bounds__(kThreads, 3) void wgrad_kernel(
         for (int p = 0; p < PL; ++p) fg[b][p] = across_fragment(s_g + p * kPlane, s, wn * 2 + b, lane);
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
-        if (a >= blocks) break;
+        if (!WEIGHTS || a >= blocks) break;
 #pragma unroll
         for (int p = 0; p < PL; ++p) fx[a][p] = across_fragment(s_x + p * kPlane, s, wk * 2 + a, lane);
 #pragma unroll
@@ -531,7 +532,8 @@ __global__ __launch_bounds__(kThreads, 3) void wgrad_kernel(
     }
   };
   const int64_t size = (int64_t)n_out * n_in;
-  if (whole) leave(reinterpret_cast<E*>(s_all), dw + it.group * size);
+  if (!WEIGHTS) {}
+  else if (whole) leave(reinterpret_cast<E*>(s_all), dw + it.group * size);
   else leave(reinterpret_cast<float*>(s_all), dw_part + it.slab * size);
   if (sum_bias) {
 #pragma unroll
@@ -1185,28 +1187,31 @@ int launch_wgrad(const void* dy, int64_t ldy, const void* x, int64_t ldx, const 
                  void* db, hipStream_t s) {
   typedef typename P::E E;
   const Split sp = split_of(sizeof(E) == 4 ? PV2_F32 : PV2_BF16, rows, groups, n_out, n_in);
-  const bool direct = sizeof(E) == 2 && aligned16(dy, ldy, n_out, 2) && aligned16(x, ldx, n_in, 2);
+  const bool weights = dw != nullptr;
+  const bool direct = sizeof(E) == 2 && weights && aligned16(dy, ldy, n_out, 2) && aligned16(x, ldx, n_in, 2);
   const int tile_cols = direct ? wgrad_cols(n_in) : kTile;
-  const int to = tiles_of(n_out, kTile), ti = tiles_of(n_in, tile_cols);
+  const int to = tiles_of(n_out, kTile), ti = weights ? tiles_of(n_in, tile_cols) : 1;
   const int64_t blocks = (sp.items + 7) / 8 * 8 * to * ti;
   PV2_REQUIRE(blocks < kMostBlocks, "grouped_linear: too many tiles");
-  const int64_t size = (int64_t)n_out * n_in;
+  const int64_t size = weights ? (int64_t)n_out * n_in : 0;
   const bool parts = rows > sp.unit;
   PV2_REQUIRE(!parts || ws, "grouped_linear: no workspace");
   float* db_part = parts ? ws + sp.slabs * size : nullptr;
 #define PV2_WGRAD(kernel)                                                                                            \
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), 0, s, (const E*)dy, ldy, (const E*)x, ldx, order, \
                      offsets, (int)rows, (int)groups, n_out, n_in, sp.unit, to, ti, (E*)dw, (E*)db, ws, db_part)
-  if constexpr (sizeof(E) == 2) {
-    if (!direct) PV2_WGRAD((wgrad_kernel<P>));
+  if (!weights) {
+    PV2_WGRAD((wgrad_kernel<P, false>));
+  } else if constexpr (sizeof(E) == 2) {
+    if (!direct) PV2_WGRAD((wgrad_kernel<P, true>));
     else if (tile_cols == 256) PV2_WGRAD((wgrad_direct_kernel<typename P::Type, 256>));
     else PV2_WGRAD((wgrad_direct_kernel<typename P::Type, 128>));
   } else {
-    PV2_WGRAD((wgrad_kernel<P>));
+    PV2_WGRAD((wgrad_kernel<P, true>));
   }
 #undef PV2_WGRAD
   if (parts) {
-    int64_t chunks = (size + kThreads - 1) / kThreads;
+    int64_t chunks = (size + (weights ? 0 : n_out) + kThreads - 1) / kThreads;
     const int64_t most = 1 + 4096 / groups;
     if (chunks > most) chunks = most;
     hipLaunchKernelGGL((join_kernel<P>), dim3((unsigned)(groups * chunks)), dim3(kThreads), 0, s, offsets, (int)rows,
@@ -1265,15 +1270,21 @@ int64_t pv2_grouped_linear_workspace_floats(int dtype, int64_t rows, int64_t gro
   return sp.slabs * ((int64_t)n_out * n_in + n_out);
 }
 
+int64_t pv2_grouped_linear_bias_workspace_floats(int dtype, int64_t rows, int64_t groups, int n_out, int n_in) {
+  if (rows < 1 || groups < 1 || n_out < 1 || n_in < 1) return 0;
+  return split_of(dtype, rows, groups, n_out, n_in).slabs * n_out;
+}
+
 int pv2_grouped_linear_grad_weight(const void* grad_out, int dtype, int64_t rows, int n_out, int64_t grad_stride,
                                    const void* x, int n_in, int64_t x_stride, int64_t groups,
                                    const int32_t* order_or_null, const int32_t* offsets, float* workspace,
-                                   void* grad_weight, void* grad_bias_or_null, pv2_stream_t stream) {
-  PV2_REQUIRE(grad_out && x && offsets && grad_weight, "grouped_linear_grad_weight: null pointer");
+                                   void* grad_weight_or_null, void* grad_bias_or_null, pv2_stream_t stream) {
+  PV2_REQUIRE(grad_out && offsets && (grad_weight_or_null ? x : grad_bias_or_null),
+              "grouped_linear_grad_weight: null pointer");
   const int st = check_shapes(rows, groups, n_out, n_in);
   if (st != PV2_OK) return st;
 #define PV2_CALL(P) (launch_wgrad<P>(grad_out, grad_stride, x, x_stride, order_or_null, offsets, rows, groups, n_out, \
-                                     n_in, workspace, grad_weight, grad_bias_or_null, (hipStream_t)stream))
+                                     n_in, workspace, grad_weight_or_null, grad_bias_or_null, (hipStream_t)stream))
   PV2_BY_TYPE(dtype, PV2_CALL, "grouped_linear_grad_weight");
 #undef PV2_CALL
 }

@@ -83,13 +83,15 @@ class _GroupedLinear(torch.autograd.Function):
             launch("pv2_grouped_linear_grad_input", x.device, ptr(gy), code, m, n, gy.stride(0), ptr(weight),
                    weight.stride(0), weight.stride(1), g, k, ptr(order), ptr(offsets), ptr(gx))
         if need_w or need_b:
-            gw = new(g, n, k)
+            gw = new(g, n, k) if need_w else None
             gb = new(g, n) if need_b else None
-            floats = _lib.lib().pv2_grouped_linear_workspace_floats(code, m, g, n, k)
+            L = _lib.lib()
+            floats = (L.pv2_grouped_linear_workspace_floats if need_w else L.pv2_grouped_linear_bias_workspace_floats)(
+                code, m, g, n, k)
             workspace = new(floats, dtype=torch.float32) if floats else None
             launch("pv2_grouped_linear_grad_weight", x.device, ptr(gy), code, m, n, gy.stride(0), ptr(x), k,
                    x.stride(0), g, ptr(order), ptr(offsets), ptr(workspace), ptr(gw), ptr(gb))
-        return gx, gw if need_w else None, gb, None, None, None
+        return gx, gw, gb, None, None, None
 
 
 def grouped_linear(x, weight, groups, bias=None):

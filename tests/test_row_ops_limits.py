@@ -37,3 +37,14 @@ def test_workspace_of_a_weight_gradient_does_not_grow_with_the_groups(dtype):
     assert L.pv2_grouped_linear_workspace_floats(1, 20000, 4096, 1024, 1024) <= 38 * (1024 * 1024 + 1024)
     for rows in (1, 255, 256):   # none can be split
         assert L.pv2_grouped_linear_workspace_floats(dtype, rows, 8, 64, 64) == 0
+
+
+def test_gradients_of_nothing():
+    """grad_weight may be null (a bias alone), not both; x is needed for the weights."""
+    L, p, n = _lib.lib(), ctypes.c_void_p(64), None
+    for x, gw, gb in ((p, n, n), (n, n, n), (n, p, p)):
+        assert L.pv2_grouped_linear_grad_weight(p, 0, 4, 3, 3, x, 8, 8, 2, n, p, n, gw, gb, n) == BADARG
+    # many rows: a bias alone has a workspace of its own size
+    assert L.pv2_grouped_linear_grad_weight(p, 0, 1 << 20, 3, 3, n, 8, 8, 2, n, p, n, n, p, n) == BADARG
+    assert 0 < L.pv2_grouped_linear_bias_workspace_floats(0, 1 << 20, 2, 3, 8) == (
+        L.pv2_grouped_linear_workspace_floats(0, 1 << 20, 2, 3, 8) // (3 * 8 + 3) * 3)
