@@ -49,6 +49,26 @@ def test_split_groups_among_many(dtype, k, n, device):
     check(sum(sizes) + 77, sizes, k, n, dtype, device)
 
 
+# Aligned 16-bit operands of so many rows take tiles of 256 x 256 where a width has an even number of 128 columns (1000, 712:
+# the last tile is partial and the last step of the reduction short) and of 128 x 128 where it is odd (1032); a group's weight
+# gradient is cut into items of 4000 to 8256 rows, whose row numbers are taken in several turns.
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k,n", [(1000, 1000), (712, 1032), (1032, 712), (1032, 1032)])
+def test_large_tiles(dtype, k, n, device):
+    torch.manual_seed(23)
+    check(33000, [1, 0, 20000, 3777, 9000], k, n, dtype, device)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [1919, 1920, 1921, 1952, 3840, 3841, 8000])
+def test_items_about_where_row_numbers_are_taken_anew(dtype, rows, device):
+    """A group's rows in one item of a weight gradient, in two at most: 1920 rows' numbers are held at a time (33000 rows and
+    72 or 36 tiles of dW make pieces of 8256 or 4160 rows)."""
+    torch.manual_seed(rows)
+    for k, n in ((1152, 1024), (1024, 1152)):
+        check(33000, [rows, 33000 - rows - 40], k, n, dtype, device)
+
+
 def test_memory_of_a_weight_gradient_with_many_groups(device):
     """4096 groups of 256 x 256: beside the gradient (0.5 GB in bf16) partial results of a few split groups only."""
     torch.manual_seed(21)
