@@ -98,7 +98,7 @@ def grouped_linear(x, weight, groups, bias=None):
     """x (M, K), weight (G, N, K), groups: RowGroups of M rows in G groups, bias (G, N) or None.  -> (M, N)."""
     if not isinstance(groups, RowGroups):
         raise TypeError("grouped_linear: groups is what row_groups.group_rows or RowGroups.from_offset returns")
-    order, offsets, n_rows = groups.order, groups.offsets, groups.n_rows
+    (order, offsets), n_rows = groups.checked("grouped_linear"), groups.n_rows
     if not launch_alone(x, weight, bias):
         return _GroupedLinear.apply(x, weight, bias, order, offsets, n_rows)
     # (products without a gradient - serving - are the launch alone)

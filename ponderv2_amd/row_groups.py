@@ -60,12 +60,18 @@ def require_index(index, what):
         raise TypeError(f"{what}: integer ids (int64 or int32) expected, got {index.dtype}")
 
 
+def _writes(t):
+    """How often a tensor was written to in place (tensors of inference mode do not count)."""
+    return None if t is None or t.is_inference() else t._version
+
+
 class RowGroups:
     """``order`` int32 (n_rows,), or None where the rows already lie in order: the rows of group 0, of group 1, ..,
     then the rows of no group; ``offsets`` int32 (n_groups + 1,): where each group's rows begin in it.  Kernels address
-    memory by both without a check, so they are made here only, by ``group_rows`` and ``from_offset``."""
+    memory by both without a check, so they are made here only, by ``group_rows`` and ``from_offset``, are not assigned to,
+    and are refused once they were written to in place."""
 
-    __slots__ = ("order", "offsets", "n_rows", "n_groups")
+    __slots__ = ("_order", "_offsets", "_n_rows", "_n_groups", "_as_made")
 
     def __init__(self, *args, **kwargs):
         raise TypeError("RowGroups are made by group_rows(index, num_groups) or RowGroups.from_offset(offset, n_rows)")
@@ -73,8 +79,23 @@ class RowGroups:
     @classmethod
     def _made(cls, order, offsets, n_rows, n_groups):
         self = object.__new__(cls)
-        self.order, self.offsets, self.n_rows, self.n_groups = order, offsets, n_rows, n_groups
+        self._order, self._offsets, self._n_rows, self._n_groups = order, offsets, n_rows, n_groups
+        self._as_made = _writes(order), _writes(offsets)
         return self
+
+    order = property(lambda self: self._order)
+    offsets = property(lambda self: self._offsets)
+    n_rows = property(lambda self: self._n_rows)
+    n_groups = property(lambda self: self._n_groups)
+
+    def checked(self, what):
+        """(order, offsets) as they were made."""
+        if (_writes(self._order), _writes(self._offsets)) != self._as_made:
+            raise RuntimeError(f"{what}: the groups' order or offsets were written to; make new ones with group_rows")
+        return self._order, self._offsets
+
+    def __reduce__(self):   # (copies are made as the original was)
+        return RowGroups._made, (*self.checked("RowGroups"), self._n_rows, self._n_groups)
 
     @classmethod
     def from_offset(cls, offset, n_rows):
