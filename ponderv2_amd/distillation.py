@@ -23,13 +23,11 @@ def _rows(t, width):
     return rows_contiguous(t if t.dim() == 2 else t.reshape(-1, width))
 
 
-def _checked(logits, teacher_index, teacher_logits):
-    """The three as matrices with contiguous rows.  Part of every pass through the operator, so that a replayed trace checks
-    and lays out the tensors of its own call."""
+def check_lists(logits, teacher_index, teacher_logits):
+    """What every form of the loss takes as lists."""
     require_index(teacher_index, "topk_distillation: teacher_index")
-    for name, t in (("logits", logits), ("teacher_logits", teacher_logits)):
-        if t.dtype not in DTYPE_CODE:
-            raise TypeError(f"topk_distillation: float32, bfloat16 or float16 {name} expected, got {t.dtype}")
+    if teacher_logits.dtype not in DTYPE_CODE:
+        raise TypeError(f"topk_distillation: float32, bfloat16 or float16 teacher_logits expected, got {teacher_logits.dtype}")
     if (logits.dim() < 1 or teacher_index.shape != teacher_logits.shape
             or teacher_index.shape[:-1] != logits.shape[:-1] or teacher_index.dim() != logits.dim()):
         raise ValueError(f"topk_distillation: logits (..., V), teacher_index and teacher_logits (..., k) expected, got "
@@ -37,9 +35,18 @@ def _checked(logits, teacher_index, teacher_logits):
     v, k = logits.shape[-1], teacher_index.shape[-1]
     if not 1 <= k <= MAX_TOP or not 1 <= v <= MAX_CLASSES:
         raise ValueError(f"topk_distillation: {v} classes (1 to {MAX_CLASSES}), {k} listed (1 to {MAX_TOP})")
+
+
+def _checked(logits, teacher_index, teacher_logits):
+    """The three as matrices with contiguous rows.  Part of every pass through the operator, so that a replayed trace checks
+    and lays out the tensors of its own call."""
+    if logits.dtype not in DTYPE_CODE:
+        raise TypeError(f"topk_distillation: float32, bfloat16 or float16 logits expected, got {logits.dtype}")
+    check_lists(logits, teacher_index, teacher_logits)
     _require_device(logits, teacher_index, teacher_logits)
     if not logits.device == teacher_index.device == teacher_logits.device:
         raise ValueError("topk_distillation: logits, teacher_index and teacher_logits are on different devices")
+    v, k = logits.shape[-1], teacher_index.shape[-1]
     return _rows(logits, v), _rows(teacher_index, k), _rows(teacher_logits, k)
 
 

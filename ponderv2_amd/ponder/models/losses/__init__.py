@@ -4,7 +4,8 @@ teacher's stored top logits."""
 import torch
 import torch.nn as nn
 
-from ponderv2_amd.distillation import MAX_TEMPERATURE, MIN_TEMPERATURE, REDUCTIONS, topk_distillation
+from ponderv2_amd.distillation import (MAX_TEMPERATURE, MIN_TEMPERATURE, REDUCTIONS, check_lists,
+                                       topk_distillation)
 
 from ...utils.registry import Registry
 
@@ -30,7 +31,8 @@ class CrossEntropyLoss(nn.Module):
 class TopLogitsDistillLoss(nn.Module):
     """Distillation from a teacher's ``k`` best classes per row (ponderv2_amd/distillation.py): ``target`` is the pair
     (teacher_index, teacher_logits), (N, k) each, index -1 where a row lists fewer.  ``from_teacher`` tells ``Criteria``
-    to hand it the teacher's lists instead of the labels.  Host tensors and float64 logits take the torch statement."""
+    to hand it the teacher's lists instead of the labels.  Host tensors and float64 logits take the torch statement, of the
+    same lists, in fp32 at least, with a gradient of the logits only."""
 
     from_teacher = True
 
@@ -48,7 +50,9 @@ class TopLogitsDistillLoss(nn.Module):
         return loss * self.loss_weight
 
     def _statement(self, pred, index, logits):
-        t = self.temperature
+        check_lists(pred, index, logits)
+        t, logits = self.temperature, logits.detach()
+        pred = pred if pred.dtype == torch.float64 else pred.float()
         ok = (index >= 0) & (index < pred.shape[-1]) & (logits != -torch.inf)
         some = ok.any(-1)
         lists = torch.where(ok, logits.to(pred.dtype) / t, -torch.inf)
