@@ -11,7 +11,7 @@ import torch
 from . import _lib
 from .embedding import rows_contiguous
 from .kernels import DTYPE_CODE, _require_device
-from .row_groups import launch, once_differentiable_backward, ptr, require_index
+from .row_groups import launch, number, once_differentiable_backward, ptr, require_index
 
 MAX_TOP = 1024
 MAX_CLASSES = (1 << 30) - 1
@@ -97,7 +97,7 @@ def topk_distillation(logits, teacher_index, teacher_logits, temperature=1.0, re
     every row's loss ("none").  The gradient, of the logits only, has their type."""
     if reduction not in REDUCTIONS:
         raise ValueError(f"topk_distillation: reduction is one of {REDUCTIONS}, got {reduction!r}")
-    temperature = float(temperature)
+    temperature = number(temperature, "topk_distillation: temperature")
     if not MIN_TEMPERATURE <= temperature <= MAX_TEMPERATURE:
         raise ValueError(f"topk_distillation: temperature {temperature} ({MIN_TEMPERATURE:g} to {MAX_TEMPERATURE:g})")
     return _TopkDistillation.apply(logits, teacher_index, teacher_logits.detach(), temperature, reduction)

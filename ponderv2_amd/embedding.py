@@ -8,7 +8,7 @@ import torch
 
 from . import _lib
 from .kernels import DTYPE_CODE, _require_device
-from .row_groups import (MAX_GROUPS, MAX_ROWS, launch, launch_alone, once_differentiable_backward, ptr,
+from .row_groups import (MAX_GROUPS, MAX_ROWS, launch, launch_alone, number, once_differentiable_backward, ptr,
                          require_index)
 
 MAX_WIDTH = (1 << 30) - 1
@@ -69,7 +69,8 @@ def rows_contiguous(t):
 
 def embedding(index, weight, scale=1.0):
     """index: int64 / int32 ids of any shape; weight (rows, C).  -> (*index.shape, C) = scale * weight[index]."""
+    scale = number(scale, "embedding: scale")
     if not launch_alone(weight):
-        return _Embedding.apply(index, weight, float(scale))
+        return _Embedding.apply(index, weight, scale)
     # (a lookup without a gradient - serving - is the launch alone)
-    return _lookup(*_checked(index, weight), float(scale), index.shape)
+    return _lookup(*_checked(index, weight), scale, index.shape)

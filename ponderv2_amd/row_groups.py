@@ -36,6 +36,13 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def number(value, what):
+    """A Python number; a tensor that asks for a gradient is refused, since none is formed for it."""
+    if isinstance(value, torch.Tensor) and value.requires_grad:
+        raise TypeError(f"{what} is a number and takes no gradient; multiply by it outside or detach it")
+    return float(value)
+
+
 def launch_alone(*tensors):
     """Whether a call may be its launch alone, past the autograd Function: none of ``tensors`` asks for a gradient, none can
     carry a tangent (the Function refuses those by name) and no trace is recorded (it would keep the empty result and not

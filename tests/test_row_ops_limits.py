@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from ponderv2_amd import _lib
+from ponderv2_amd.distillation import topk_distillation
 from ponderv2_amd.embedding import embedding
 
 BADARG = -1
@@ -48,3 +49,18 @@ def test_gradients_of_nothing():
     assert L.pv2_grouped_linear_grad_weight(p, 0, 1 << 20, 3, 3, n, 8, 8, 2, n, p, n, n, p, n) == BADARG
     assert 0 < L.pv2_grouped_linear_bias_workspace_floats(0, 1 << 20, 2, 3, 8) == (
         L.pv2_grouped_linear_workspace_floats(0, 1 << 20, 2, 3, 8) // (3 * 8 + 3) * 3)
+
+
+def test_scales_and_temperatures_take_no_gradient():
+    """A learnable one is refused: its gradient would be lost."""
+    learnable = torch.tensor(2.0, requires_grad=True)
+    ids, lists = torch.zeros(4, dtype=torch.int64), torch.zeros(4, 2)
+    with pytest.raises(TypeError, match="scale is a number and takes no gradient"):
+        embedding(ids, torch.zeros(3, 8), learnable)
+    with pytest.raises(TypeError, match="temperature is a number and takes no gradient"):
+        topk_distillation(torch.zeros(4, 8), lists.long(), lists, learnable)
+    for number in (2, 2.0, torch.tensor(2.0), learnable.detach()):
+        for call in (lambda: embedding(ids, torch.zeros(3, 8), number),
+                     lambda: topk_distillation(torch.zeros(4, 8), lists.long(), lists, number)):
+            with pytest.raises(RuntimeError, match="no CPU fallback"):
+                call()
