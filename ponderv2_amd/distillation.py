@@ -28,13 +28,14 @@ def check_lists(logits, teacher_index, teacher_logits):
     require_index(teacher_index, "topk_distillation: teacher_index")
     if teacher_logits.dtype not in DTYPE_CODE:
         raise TypeError(f"topk_distillation: float32, bfloat16 or float16 teacher_logits expected, got {teacher_logits.dtype}")
-    if (logits.dim() < 1 or teacher_index.shape != teacher_logits.shape
-            or teacher_index.shape[:-1] != logits.shape[:-1] or teacher_index.dim() != logits.dim()):
+    shape, lists = logits.shape, teacher_index.shape
+    if len(shape) < 1 or teacher_logits.shape != lists or len(lists) != len(shape) or lists[:-1] != shape[:-1]:
         raise ValueError(f"topk_distillation: logits (..., V), teacher_index and teacher_logits (..., k) expected, got "
-                         f"{tuple(logits.shape)}, {tuple(teacher_index.shape)}, {tuple(teacher_logits.shape)}")
-    v, k = logits.shape[-1], teacher_index.shape[-1]
+                         f"{tuple(shape)}, {tuple(lists)}, {tuple(teacher_logits.shape)}")
+    v, k = shape[-1], lists[-1]
     if not 1 <= k <= MAX_TOP or not 1 <= v <= MAX_CLASSES:
         raise ValueError(f"topk_distillation: {v} classes (1 to {MAX_CLASSES}), {k} listed (1 to {MAX_TOP})")
+    return v, k
 
 
 def _checked(logits, teacher_index, teacher_logits):
@@ -42,53 +43,51 @@ def _checked(logits, teacher_index, teacher_logits):
     and lays out the tensors of its own call."""
     if logits.dtype not in DTYPE_CODE:
         raise TypeError(f"topk_distillation: float32, bfloat16 or float16 logits expected, got {logits.dtype}")
-    check_lists(logits, teacher_index, teacher_logits)
+    v, k = check_lists(logits, teacher_index, teacher_logits)
     _require_device(logits, teacher_index, teacher_logits)
     if not logits.device == teacher_index.device == teacher_logits.device:
         raise ValueError("topk_distillation: logits, teacher_index and teacher_logits are on different devices")
-    v, k = logits.shape[-1], teacher_index.shape[-1]
     return _rows(logits, v), _rows(teacher_index, k), _rows(teacher_logits, k)
 
 
 class _TopkDistillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, index, teacher, temperature, reduction):
-        lead, ctx.dtype = logits.shape[:-1], logits.dtype
+        shape = logits.shape
         logits, index, teacher = _checked(logits, index, teacher)
-        m, v, k = int(logits.shape[0]), int(logits.shape[1]), int(index.shape[1])   # (tensors while a trace is recorded)
-        ctx.shape = (*lead, v)
+        (m, v), k = logits.shape, index.shape[1]
         device = logits.device
+        ctx.how = (temperature, reduction, None if len(shape) == 2 else shape)
         if m == 0:   # nothing to launch: an exact zero
-            return torch.zeros(lead if reduction == "none" else (), dtype=torch.float32, device=device)
+            ctx.save_for_backward(logits, index, teacher, None)
+            return torch.zeros(shape[:-1] if reduction == "none" else (), dtype=torch.float32, device=device)
         # the rows' statistics, their number, and scratch
         saved = torch.empty(2 * m + 1 + _lib.lib().pv2_topk_distill_workspace_floats(m, v, k), dtype=torch.float32,
                             device=device)
         loss = torch.empty((), dtype=torch.float32, device=device)
-        row_loss = torch.empty(lead, dtype=torch.float32, device=device) if reduction == "none" else None
+        row_loss = torch.empty(shape[:-1], dtype=torch.float32, device=device) if reduction == "none" else None
         stats = ptr(saved)
-        count = stats + 8 * m
+        count = stats + 8 * int(m)   # (sizes are tensors while a trace is recorded)
         launch("pv2_topk_distill_forward", device, ptr(logits), DTYPE_CODE[logits.dtype], m, v, logits.stride(0),
                ptr(index), index.dtype == torch.int64, index.stride(0), ptr(teacher), DTYPE_CODE[teacher.dtype],
                teacher.stride(0), k, temperature, reduction == "mean", count + 4, stats, ptr(row_loss), ptr(loss), count)
         ctx.save_for_backward(logits, index, teacher, saved)
-        ctx.how = (temperature, reduction)
         return loss if row_loss is None else row_loss
 
     @once_differentiable_backward
     def backward(ctx, up):
-        if 0 in ctx.shape:
-            return up.new_zeros(ctx.shape, dtype=ctx.dtype), None, None, None, None
         logits, index, teacher, saved = ctx.saved_tensors
-        temperature, reduction = ctx.how
+        temperature, reduction, shape = ctx.how
         (m, v), k = logits.shape, index.shape[1]
         up = up.contiguous()
         grad = torch.empty((m, v), dtype=logits.dtype, device=logits.device)
-        stats = ptr(saved)
-        launch("pv2_topk_distill_backward", logits.device, ptr(logits), DTYPE_CODE[logits.dtype], m, v,
-               logits.stride(0), ptr(index), index.dtype == torch.int64, index.stride(0), ptr(teacher),
-               DTYPE_CODE[teacher.dtype], teacher.stride(0), k, temperature, stats, ptr(up), reduction == "none",
-               stats + 8 * m if reduction == "mean" else None, ptr(grad))
-        return grad.view(ctx.shape), None, None, None, None
+        if m:
+            stats = ptr(saved)
+            launch("pv2_topk_distill_backward", logits.device, ptr(logits), DTYPE_CODE[logits.dtype], m, v,
+                   logits.stride(0), ptr(index), index.dtype == torch.int64, index.stride(0), ptr(teacher),
+                   DTYPE_CODE[teacher.dtype], teacher.stride(0), k, temperature, stats, ptr(up), reduction == "none",
+                   stats + 8 * m if reduction == "mean" else None, ptr(grad))
+        return grad if shape is None else grad.view(shape), None, None, None, None
 
 
 def topk_distillation(logits, teacher_index, teacher_logits, temperature=1.0, reduction="mean"):

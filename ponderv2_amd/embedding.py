@@ -14,13 +14,14 @@ from .row_groups import (MAX_GROUPS, MAX_ROWS, launch, launch_alone, number, onc
 MAX_WIDTH = (1 << 30) - 1
 
 
-def _checked(index, weight):
-    """The ids as one list and the table with contiguous rows.  Part of every pass through the operator, so that a replayed
-    trace checks and lays out the tensors of its own call."""
+def _lookup(index, weight, scale):
+    """(the rows, the ids as one list).  Checks and layout are part of it, so that a replayed trace checks and lays out the
+    tensors of its own call."""
     require_index(index, "embedding")
-    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+    if weight.dim() != 2 or 0 in weight.shape:
         raise ValueError(f"embedding: weight is (rows, channels), got {tuple(weight.shape)}")
-    if index.numel() > MAX_ROWS or weight.shape[0] > MAX_GROUPS or weight.shape[1] > MAX_WIDTH:
+    n, (rows, c) = index.numel(), weight.shape
+    if n > MAX_ROWS or rows > MAX_GROUPS or c > MAX_WIDTH:
         raise ValueError(f"embedding: up to {MAX_ROWS} indices, {MAX_GROUPS} rows and {MAX_WIDTH} channels")
     if weight.dtype not in DTYPE_CODE:
         raise TypeError(f"embedding: float32, bfloat16 or float16 weight expected, got {weight.dtype}")
@@ -28,25 +29,21 @@ def _checked(index, weight):
     if index.device != weight.device:
         raise ValueError(f"embedding: index on {index.device}, weight on {weight.device}")
     flat = index if index.dim() == 1 and index.is_contiguous() else index.reshape(-1).contiguous()
-    return flat, rows_contiguous(weight)
-
-
-def _lookup(flat, weight, scale, shape):
-    n, (rows, c) = flat.numel(), weight.shape
-    y = torch.empty((*shape, c), dtype=weight.dtype, device=weight.device)
+    weight = rows_contiguous(weight)
+    y = torch.empty((*index.shape, c), dtype=weight.dtype, device=weight.device)
     if n:
         launch("pv2_embedding_forward", weight.device, ptr(flat), flat.dtype == torch.int64, n, ptr(weight),
                DTYPE_CODE[weight.dtype], rows, c, weight.stride(0), scale, ptr(y))
-    return y
+    return y, flat
 
 
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, index, weight, scale):
-        flat, weight = _checked(index, weight)
+        y, flat = _lookup(index, weight, scale)
         ctx.save_for_backward(flat)
         ctx.table = (*weight.shape, scale)
-        return _lookup(flat, weight, scale, index.shape)
+        return y
 
     @once_differentiable_backward
     def backward(ctx, gy):
@@ -69,8 +66,8 @@ def rows_contiguous(t):
 
 def embedding(index, weight, scale=1.0):
     """index: int64 / int32 ids of any shape; weight (rows, C).  -> (*index.shape, C) = scale * weight[index]."""
-    scale = number(scale, "embedding: scale")
+    scale = scale if type(scale) is float else number(scale, "embedding: scale")
     if not launch_alone(weight):
         return _Embedding.apply(index, weight, scale)
     # (a lookup without a gradient - serving - is the launch alone)
-    return _lookup(*_checked(index, weight), scale, index.shape)
+    return _lookup(index, weight, scale)[0]

@@ -25,46 +25,43 @@ def _weight_rows(w):
     return w if w.stride(2) == 1 or w.shape[2] == 1 else w.contiguous()
 
 
-def _checked(x, weight, bias, order, offsets, n_rows):
-    """The operands with contiguous rows.  Part of every pass through the operator, so that a replayed trace checks and lays
-    out the tensors of its own call.  n_rows: of groups without an order."""
+def _products(x, weight, bias, order, offsets, n_rows):
+    """(the products, x and weight as the kernels take them).  Checks and layout are part of it, so that a replayed trace
+    checks and lays out the tensors of its own call.  n_rows: of groups without an order."""
     if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2]:
         raise ValueError(f"grouped_linear: x (M, K) and weight (G, N, K) expected, got {tuple(x.shape)} and "
                          f"{tuple(weight.shape)}")
-    g, n, k = weight.shape
+    (m, k), (g, n, _) = x.shape, weight.shape
     n_rows, n_groups = int(n_rows) if order is None else order.numel(), offsets.numel() - 1
-    if n_rows != x.shape[0] or n_groups != g:
-        raise ValueError(f"grouped_linear: {x.shape[0]} rows and {g} weights, but groups of {n_rows} rows in "
+    if n_rows != m or n_groups != g:
+        raise ValueError(f"grouped_linear: {m} rows and {g} weights, but groups of {n_rows} rows in "
                          f"{n_groups} groups")
     if bias is not None and tuple(bias.shape) != (g, n):
         raise ValueError(f"grouped_linear: bias is (G, N) = {(g, n)}, got {tuple(bias.shape)}")
-    if min(n, k) < 1 or max(n, k) > MAX_WIDTH or x.shape[0] > MAX_ROWS or g > MAX_GROUPS:
+    if min(n, k) < 1 or max(n, k) > MAX_WIDTH or m > MAX_ROWS or g > MAX_GROUPS:
         raise ValueError(f"grouped_linear: widths 1 to {MAX_WIDTH}, up to {MAX_ROWS} rows and {MAX_GROUPS} groups")
-    tensors = [x, weight] + ([] if bias is None else [bias])
-    if x.dtype not in DTYPE_CODE or any(t.dtype != x.dtype for t in tensors):
+    dtype, device = x.dtype, x.device
+    if dtype not in DTYPE_CODE or weight.dtype != dtype or bias is not None and bias.dtype != dtype:
         raise TypeError("grouped_linear: x, weight and bias are all float32, all bfloat16 or all float16, got "
-                        + ", ".join(str(t.dtype) for t in tensors))
-    _require_device(*tensors)
-    if any(t.device != x.device for t in tensors + [offsets]):
+                        + ", ".join(str(t.dtype) for t in (x, weight, bias) if t is not None))
+    _require_device(x, weight, bias)
+    if weight.device != device or offsets.device != device or bias is not None and bias.device != device:
         raise ValueError("grouped_linear: x, weight, bias and groups are on different devices")
-    return rows_contiguous(x), _weight_rows(weight), None if bias is None else bias.contiguous()
-
-
-def _products(x, weight, bias, order, offsets):
-    (m, k), (g, n, _) = x.shape, weight.shape
-    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    x, weight = rows_contiguous(x), _weight_rows(weight)
+    bias = None if bias is None else bias.contiguous()
+    y = torch.empty((m, n), dtype=dtype, device=device)
     if m:
-        launch("pv2_grouped_linear_forward", x.device, ptr(x), DTYPE_CODE[x.dtype], m, k, x.stride(0), ptr(weight),
+        launch("pv2_grouped_linear_forward", device, ptr(x), DTYPE_CODE[dtype], m, k, x.stride(0), ptr(weight),
                weight.stride(0), weight.stride(1), g, n, ptr(bias), ptr(order), ptr(offsets), ptr(y))
-    return y
+    return y, x, weight
 
 
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, order, offsets, n_rows):
-        x, weight, bias = _checked(x, weight, bias, order, offsets, n_rows)
+        y, x, weight = _products(x, weight, bias, order, offsets, n_rows)
         ctx.save_for_backward(x, weight, order, offsets)
-        return _products(x, weight, bias, order, offsets)
+        return y
 
     @once_differentiable_backward
     def backward(ctx, gy):
@@ -98,8 +95,9 @@ def grouped_linear(x, weight, groups, bias=None):
     """x (M, K), weight (G, N, K), groups: RowGroups of M rows in G groups, bias (G, N) or None.  -> (M, N)."""
     if not isinstance(groups, RowGroups):
         raise TypeError("grouped_linear: groups is what row_groups.group_rows or RowGroups.from_offset returns")
-    (order, offsets), n_rows = groups.checked("grouped_linear"), groups.n_rows
+    order, offsets = groups.checked("grouped_linear")
+    n_rows = groups.n_rows if order is None else None
     if not launch_alone(x, weight, bias):
         return _GroupedLinear.apply(x, weight, bias, order, offsets, n_rows)
     # (products without a gradient - serving - are the launch alone)
-    return _products(*_checked(x, weight, bias, order, offsets, n_rows), order, offsets)
+    return _products(x, weight, bias, order, offsets, n_rows)[0]

@@ -15,6 +15,8 @@ from .kernels import _raw_stream, _require_device
 MAX_ROWS = (1 << 31) - 4097
 MAX_GROUPS = 1 << 30
 
+_tracing_state = torch._C._get_tracing_state
+
 
 def launch(name, device, *args):
     """The entry point ``name`` on the current stream of ``device``, whichever device is current.  Tensors are passed by
@@ -47,8 +49,13 @@ def launch_alone(*tensors):
     """Whether a call may be its launch alone, past the autograd Function: none of ``tensors`` asks for a gradient, none can
     carry a tangent (the Function refuses those by name) and no trace is recorded (it would keep the empty result and not
     the launch that fills it)."""
-    return (forward_ad._current_level < 0 and torch._C._get_tracing_state() is None
-            and not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)))
+    if forward_ad._current_level >= 0 or _tracing_state() is not None:
+        return False
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return False
+    return True
 
 
 def once_differentiable_backward(fn):
@@ -67,18 +74,13 @@ def require_index(index, what):
         raise TypeError(f"{what}: integer ids (int64 or int32) expected, got {index.dtype}")
 
 
-def _writes(t):
-    """How often a tensor was written to in place (tensors of inference mode do not count)."""
-    return None if t is None or t.is_inference() else t._version
-
-
 class RowGroups:
     """``order`` int32 (n_rows,), or None where the rows already lie in order: the rows of group 0, of group 1, ..,
     then the rows of no group; ``offsets`` int32 (n_groups + 1,): where each group's rows begin in it.  Kernels address
     memory by both without a check, so they are made here only, by ``group_rows`` and ``from_offset``, are not assigned to,
     and are refused once they were written to in place."""
 
-    __slots__ = ("_order", "_offsets", "_n_rows", "_n_groups", "_as_made")
+    __slots__ = ("_order", "_offsets", "_n_rows", "_n_groups")
 
     def __init__(self, *args, **kwargs):
         raise TypeError("RowGroups are made by group_rows(index, num_groups) or RowGroups.from_offset(offset, n_rows)")
@@ -87,8 +89,11 @@ class RowGroups:
     def _made(cls, order, offsets, n_rows, n_groups):
         self = object.__new__(cls)
         self._order, self._offsets, self._n_rows, self._n_groups = order, offsets, n_rows, n_groups
-        self._as_made = _writes(order), _writes(offsets)
         return self
+
+    @classmethod
+    def _copied(cls, order, offsets, n_rows, n_groups):
+        return cls._made(None if order is None else order.clone(), offsets.clone(), n_rows, n_groups)
 
     order = property(lambda self: self._order)
     offsets = property(lambda self: self._offsets)
@@ -96,19 +101,24 @@ class RowGroups:
     n_groups = property(lambda self: self._n_groups)
 
     def checked(self, what):
-        """(order, offsets) as they were made."""
-        if (_writes(self._order), _writes(self._offsets)) != self._as_made:
+        """(order, offsets), which nothing has written to since they were made."""
+        order, offsets = self._order, self._offsets
+        try:
+            written = offsets._version or order is not None and order._version
+        except RuntimeError:   # (tensors of inference mode do not count their writes)
+            written = False
+        if written:
             raise RuntimeError(f"{what}: the groups' order or offsets were written to; make new ones with group_rows")
-        return self._order, self._offsets
+        return order, offsets
 
-    def __reduce__(self):   # (copies are made as the original was)
-        return RowGroups._made, (*self.checked("RowGroups"), self._n_rows, self._n_groups)
+    def __reduce__(self):
+        return RowGroups._copied, (*self.checked("RowGroups"), self._n_rows, self._n_groups)
 
     @classmethod
     def from_offset(cls, offset, n_rows):
         """Rows 0 .. offset[0] - 1 are group 0's, offset[0] .. offset[1] - 1 group 1's, ..; rows behind the last
         offset belong to no group."""
-        offsets = _from_offset(offset, n_rows) if launch_alone() else _FromOffset.apply(offset, n_rows)
+        offsets = (_from_offset if _tracing_state() is None else _FromOffset.apply)(offset, n_rows)
         return cls._made(None, offsets, n_rows, offset.numel())
 
 
@@ -161,5 +171,5 @@ class _GroupRows(torch.autograd.Function):
 def group_rows(index, num_groups):
     """index: integer ids of the rows (any shape, read as one list).  -> RowGroups with the stable order by id; rows
     whose id is outside 0 .. num_groups - 1 (padding, unlabelled points at -1) belong to no group."""
-    order, offsets = (_group_rows if launch_alone() else _GroupRows.apply)(index, num_groups)
+    order, offsets = (_group_rows if _tracing_state() is None else _GroupRows.apply)(index, num_groups)
     return RowGroups._made(order, offsets, index.numel(), num_groups)
