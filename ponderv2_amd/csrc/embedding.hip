@@ -391,6 +391,7 @@ int pv2_embedding_backward(const void* index, int index_is_64, int64_t n, const 
   PV2_REQUIRE(grad_weight && workspace && (n == 0 || (index && grad_out)), "embedding_backward: null pointer");
   PV2_REQUIRE(n >= 0 && rows > 0 && c > 0 && c < kMaxWidth && grad_row_stride >= 0, "embedding_backward: bad shape");
   PV2_REQUIRE((uintptr_t)workspace % 32 == 0, "embedding_backward: workspace not aligned to 32 bytes");
+  PV2_REQUIRE(dtype == PV2_F32 || dtype == PV2_BF16 || dtype == PV2_F16, "embedding_backward: bad element type");
   hipStream_t s = (hipStream_t)stream;
   const Layout l = layout_of(n, rows, c);
   const int st = pv2_row_groups(index, index_is_64, n, rows, workspace + l.order, workspace + l.offsets,
@@ -409,7 +410,7 @@ int pv2_embedding_backward(const void* index, int index_is_64, int64_t n, const 
       return vec ? backward<H16, 8>(workspace, l, n, rows, grad_out, c, grad_row_stride, scale, grad_weight, s)
                  : backward<H16, 1>(workspace, l, n, rows, grad_out, c, grad_row_stride, scale, grad_weight, s);
   }
-  PV2_REQUIRE(false, "embedding_backward: bad element type");
+  return PV2_E_BADARG;
 }
 
 }  // extern "C"

@@ -64,3 +64,9 @@ def test_scales_and_temperatures_take_no_gradient():
                      lambda: topk_distillation(torch.zeros(4, 8), lists.long(), lists, number)):
             with pytest.raises(RuntimeError, match="no CPU fallback"):
                 call()
+
+
+def test_an_unknown_type_is_refused_before_the_sort():
+    L, p, n = _lib.lib(), ctypes.c_void_p(64), None
+    for dtype in (-1, 3, 7):
+        assert L.pv2_embedding_backward(p, 1, 4, p, dtype, 3, 8, 8, 1.0, p, p, n) == BADARG
