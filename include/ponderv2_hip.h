@@ -1091,7 +1091,7 @@ int pv2_grouped_linear_grad_input(const void* grad_out, int dtype, int64_t rows,
                                   int64_t groups, int n_in, const int32_t* order_or_null, const int32_t* offsets,
                                   void* grad_x, pv2_stream_t stream);
 int64_t pv2_grouped_linear_workspace_floats(int dtype, int64_t rows, int64_t groups, int n_out, int n_in);
-int64_t pv2_grouped_linear_bias_workspace_floats(int dtype, int64_t rows, int64_t groups, int n_out, int n_in);
+int64_t pv2_grouped_linear_bias_workspace_floats(int dtype, int64_t rows, int64_t groups, int n_out);
 int pv2_grouped_linear_grad_weight(const void* grad_out, int dtype, int64_t rows, int n_out, int64_t grad_stride,
                                    const void* x, int n_in, int64_t x_stride, int64_t groups,
                                    const int32_t* order_or_null, const int32_t* offsets, float* workspace,

@@ -263,7 +263,7 @@ SIGNATURES["pv2_grouped_linear_forward"] = (
 SIGNATURES["pv2_grouped_linear_grad_input"] = (
     c_int, [_P, c_int, c_int64, c_int, c_int64, _P, c_int64, c_int64, c_int64, c_int, _P, _P, _P, _P])
 SIGNATURES["pv2_grouped_linear_workspace_floats"] = (c_int64, [c_int, c_int64, c_int64, c_int, c_int])
-SIGNATURES["pv2_grouped_linear_bias_workspace_floats"] = (c_int64, [c_int, c_int64, c_int64, c_int, c_int])
+SIGNATURES["pv2_grouped_linear_bias_workspace_floats"] = (c_int64, [c_int, c_int64, c_int64, c_int])
 SIGNATURES["pv2_grouped_linear_grad_weight"] = (
     c_int, [_P, c_int, c_int64, c_int, c_int64, _P, c_int, c_int64, c_int64, _P, _P, _P, _P, _P, _P])
 SIGNATURES["pv2_topk_distill_workspace_floats"] = (c_int64, [c_int64, c_int, c_int])

@@ -419,7 +419,7 @@ __global__ __launch_bounds__(kThreads, 3) void rows_kernel(
 }
 
 // dW[g][n][k] over one item's rows.  The item is the whole group: written in the weights' type; else fp32 partials.
-// WEIGHTS false: db alone, the same sums in the same order; x is not read (tiles_in is 1).
+// WEIGHTS false: db alone, x is not read (tiles_in is 1, items as for one column of x).
 template <class P, bool WEIGHTS>
 __global__ __launch_bounds__(kThreads, 3) void wgrad_kernel(
     const typename P::E* __restrict__ dy, int64_t ldy, const typename P::E* __restrict__ x, int64_t ldx,
@@ -1186,8 +1186,8 @@ int launch_wgrad(const void* dy, int64_t ldy, const void* x, int64_t ldx, const 
                  const int32_t* offsets, int64_t rows, int64_t groups, int n_out, int n_in, float* ws, void* dw,
                  void* db, hipStream_t s) {
   typedef typename P::E E;
-  const Split sp = split_of(sizeof(E) == 4 ? PV2_F32 : PV2_BF16, rows, groups, n_out, n_in);
   const bool weights = dw != nullptr;
+  const Split sp = split_of(sizeof(E) == 4 ? PV2_F32 : PV2_BF16, rows, groups, n_out, weights ? n_in : 1);
   const bool direct = sizeof(E) == 2 && weights && aligned16(dy, ldy, n_out, 2) && aligned16(x, ldx, n_in, 2);
   const int tile_cols = direct ? wgrad_cols(n_in) : kTile;
   const int to = tiles_of(n_out, kTile), ti = weights ? tiles_of(n_in, tile_cols) : 1;
@@ -1270,9 +1270,9 @@ int64_t pv2_grouped_linear_workspace_floats(int dtype, int64_t rows, int64_t gro
   return sp.slabs * ((int64_t)n_out * n_in + n_out);
 }
 
-int64_t pv2_grouped_linear_bias_workspace_floats(int dtype, int64_t rows, int64_t groups, int n_out, int n_in) {
-  if (rows < 1 || groups < 1 || n_out < 1 || n_in < 1) return 0;
-  return split_of(dtype, rows, groups, n_out, n_in).slabs * n_out;
+int64_t pv2_grouped_linear_bias_workspace_floats(int dtype, int64_t rows, int64_t groups, int n_out) {
+  if (rows < 1 || groups < 1 || n_out < 1) return 0;
+  return split_of(dtype, rows, groups, n_out, 1).slabs * n_out;
 }
 
 int pv2_grouped_linear_grad_weight(const void* grad_out, int dtype, int64_t rows, int n_out, int64_t grad_stride,

@@ -83,8 +83,8 @@ class _GroupedLinear(torch.autograd.Function):
             gw = new(g, n, k) if need_w else None
             gb = new(g, n) if need_b else None
             L = _lib.lib()
-            floats = (L.pv2_grouped_linear_workspace_floats if need_w else L.pv2_grouped_linear_bias_workspace_floats)(
-                code, m, g, n, k)
+            floats = (L.pv2_grouped_linear_workspace_floats(code, m, g, n, k) if need_w
+                      else L.pv2_grouped_linear_bias_workspace_floats(code, m, g, n))
             workspace = new(floats, dtype=torch.float32) if floats else None
             launch("pv2_grouped_linear_grad_weight", x.device, ptr(gy), code, m, n, gy.stride(0), ptr(x), k,
                    x.stride(0), g, ptr(order), ptr(offsets), ptr(workspace), ptr(gw), ptr(gb))

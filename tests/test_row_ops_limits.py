@@ -47,7 +47,7 @@ def test_gradients_of_nothing():
         assert L.pv2_grouped_linear_grad_weight(p, 0, 4, 3, 3, x, 8, 8, 2, n, p, n, gw, gb, n) == BADARG
     # many rows: a bias alone has a workspace of its own size
     assert L.pv2_grouped_linear_grad_weight(p, 0, 1 << 20, 3, 3, n, 8, 8, 2, n, p, n, n, p, n) == BADARG
-    assert 0 < L.pv2_grouped_linear_bias_workspace_floats(0, 1 << 20, 2, 3, 8) == (
+    assert 0 < L.pv2_grouped_linear_bias_workspace_floats(0, 1 << 20, 2, 3) == (
         L.pv2_grouped_linear_workspace_floats(0, 1 << 20, 2, 3, 8) // (3 * 8 + 3) * 3)
 
 
