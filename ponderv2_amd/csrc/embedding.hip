@@ -12,9 +12,9 @@
 //   rows     every other row of dW: zeros, or the sum of at most 33 partial rows of pieces, or of those of blocks.
 // So all waves have the same work and few dependent reads, whatever the ids' frequencies.  (One wave per row of dW instead
 // of per piece: the ids of 2 .. 32 tokens, neighbours in a vocabulary, made a few waves last 80 us.)
-// Measured on MI355X (copy 5.1 TB/s): 92 001 ids over 36 rows of 512 fp32, lookup 41 us (188 MB written), gradient 80 us
-// (pieces 53 - 188 MB read while the lookup's writes still drain -, sort 13); 32 768 ids over 65 536 rows of 1024 bf16,
-// lookup 26 us, gradient 95 us (sort 32, pieces 25, rows 30: 112 MB of zeros).
+// Measured on MI355X (copy 5.1 TB/s): 92 001 ids over 36 rows of 512 fp32, lookup 32 us (188 MB written), gradient 84 us
+// (pieces 54 - 188 MB read while the lookup's writes still drain -, sort 13, joins 13); 32 768 ids over 65 536 rows of 1024 bf16,
+// lookup 26 us, gradient 94 us (sort 33, pieces 21, blocks 8, rows 32: 112 MB of zeros).
 #include <type_traits>
 
 #include "common.h"

@@ -13,20 +13,24 @@
 // rows_direct_kernel   the same for aligned 16-bit operands, memory -> LDS directly: 256 x 256 (waves of 64 x 128) or
 //                      128 x 128.
 // wgrad_kernel,        dW and db: a 128 x 128 (256) tile of one group's dW; long groups are split over rows into items
-// wgrad_direct_kernel  whose fp32 partial results a second launch adds in order (no atomics).  db is summed from the
-//                      fragments of dY.
+// wgrad_direct_kernel  whose fp32 partial results a second launch adds in order (no atomics); a group of one item has
+//                      none.  db is summed from the fragments of dY, alone where dW is not asked for.
 // few_rows_kernel      Y for a handful of rows (serving): bound by reading the weights once; 16 output columns per
 //                      workgroup, the reduction split over its four waves, operands straight from memory to registers.
 //
 // Measured on MI355X (a library product of 8192^3 reaches 1374 TFLOP/s in bf16, of 4096^3 137 in fp32):
-//   bf16, 16 groups of 2048 rows, 1024 x 1024   Y 75 us (918 TFLOP/s), dX 80, dW 102; ragged groups 92, 100, 109
+//   bf16, 16 groups of 2048 rows, 1024 x 1024   Y 77 us (892 TFLOP/s), dX 87 - 92, dW and db 102 - 105, db alone 26;
+//                                               ragged groups 98 - 106, 102 - 111, 110 - 117, 28
 //                                               (one library product of all rows with one weight: 58)
-//   bf16, one group of 32 768, 4096 -> 1024     Y 280 us (983 TFLOP/s)
-//   fp32, the same 16 groups                    Y 365 us (188 TFLOP/s), dX 370, dW 395 (library: 482, 562)
-//   fp32, 3 groups of 92 417 rows, 96 -> 512    Y 77 us, dX 72, dW 81 (library, one weight: 125)
-//   bf16, 8 rows over 16 groups, 1024 -> 2048   9 us (27 MB of weights: 5 us at the rate of a copy)
+//   bf16, one group of 32 768, 4096 -> 1024     Y 280 - 307 us, dX 325, dW and db 1180 (256 workgroups in all), db alone 27
+//   bf16, 16 ragged groups, 1023 x 1023         Y 137 us, dX 176, dW and db 322, db alone 50 (rows not aligned)
+//   fp32, 16 groups of 2048, 1024 x 1024        Y 365 - 390 us (180 TFLOP/s), dX 370, dW and db 455, db alone 28
+//                                               (library: Y 482, dX 562)
+//   fp32, 3 groups of 92 417 rows, 96 -> 512    Y 75 us, dX 80, dW and db 95, of them 11 to join, db alone 41; within a
+//                                               training step 90, 78, 103 (library, one weight: Y 125)
+//   8 rows over 16 groups, 1024 -> 2048         bf16 Y 9 us (27 MB of weights: 5 us at the rate of a copy), dX 28; fp32 15, 113
 // What bounds the 16-bit products: loads into LDS and products overlap only in part.  Alone, with everything else taken out,
-// products take 157 us and loads 196 of the 280 (4096 -> 1024); three stages of 256 x 128 or 32-deep steps three ahead, which
+// products take 157 us and loads 196 of 280 (4096 -> 1024); three stages of 256 x 128 or 32-deep steps three ahead, which
 // wait less but load more, are slower (364 and 350).  The 256 CUs hold 512 tiles of 256 x 256 in two rounds; a few more, as
 // ragged groups make, cost most of a third.
 #include <type_traits>

@@ -295,7 +295,8 @@ __global__ __launch_bounds__(kSmallThreads) void small_kernel(Source src, int n,
     for (int g = tid; g <= n_groups; g += kSmallThreads) offsets[g] = pv2::lower_bound(s_key[cur], n, g);
 }
 
-// cumulative row counts (B,) -> offsets [B + 1], never decreasing and within 0 .. n whatever the counts hold
+// cumulative row counts (B,) -> offsets [B + 1], never decreasing and within 0 .. n whatever the counts hold.  One wave: the
+// scenes of a batch are few (up to 64: 1.5 us; 1000 take 7, 4096 23, 65536 355)
 __global__ __launch_bounds__(64) void offsets_from_counts_kernel(const void* cumulative, int is64, int n_groups,
                                                                  int64_t n, int32_t* __restrict__ offsets) {
   const int lane = threadIdx.x;
