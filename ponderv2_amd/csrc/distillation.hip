@@ -12,7 +12,7 @@
 //   V <= 512       a row per 4 .. 64 lanes of a wave, held in registers;
 //   larger V       a workgroup per row, or - few rows - several per row and a second launch that joins their statistics.
 // Sums over rows are formed from per-workgroup sums in a fixed order: no atomics.
-// Measured on MI355X: 4096 x 65 537 bf16, k = 32: forward 135 - 149 us, backward 206 - 210 us - 1.61 GB at 4.6 TB/s, where a copy
+// Measured on MI355X: 4096 x 65 537 bf16, k = 32: forward 135 - 144 us, backward 206 - 210 us - 1.61 GB at 4.6 TB/s, where a copy
 // reaches 5.1; without the exponentials the forward pass takes 142 us, without its lists 140.  92 001 x 25 fp32: 9 + 3 and
 // 13 us; one row of 131 072: 11 and 7 us.
 #include <type_traits>
