@@ -16,6 +16,7 @@ MAX_ROWS = (1 << 31) - 4097
 MAX_GROUPS = 1 << 30
 
 _tracing_state = torch._C._get_tracing_state
+_compiling = torch.compiler.is_compiling
 
 
 def launch(name, device, *args):
@@ -103,8 +104,8 @@ class RowGroups:
     def checked(self, what):
         """(order, offsets), which nothing has written to since they were made."""
         order, offsets = self._order, self._offsets
-        try:
-            written = offsets._version or order is not None and order._version
+        try:   # (while torch.compile looks at it the counts are symbols: nothing to decide by)
+            written = not _compiling() and (offsets._version or order is not None and order._version)
         except RuntimeError:   # (tensors of inference mode do not count their writes)
             written = False
         if written:

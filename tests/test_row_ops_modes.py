@@ -242,3 +242,26 @@ def test_a_traced_distillation_replays(where, reduction):
     empty = traced(torch.zeros(0, 9, device=where), torch.zeros(0, 3, dtype=torch.int64, device=where),
                    torch.zeros(0, 3, device=where))
     assert empty.shape == ((0,) if reduction == "none" else ()) and not empty.any()
+
+
+# ------------------------------------------------------------------------------------------ torch.compile
+@pytest.mark.parametrize("train", [False, True])
+def test_compiled_callers(where, train):
+    """The operators run as they are inside a function that torch.compile has taken (backend "eager": nothing is generated)."""
+    x, w, b, index = problem(20, 3, 8, 4, where)
+    groups = group_rows(index, 3)
+    teacher = torch.randint(-1, 4, (20, 2), device=where), torch.randn(20, 2, device=where)
+
+    def step(x, w, b, index):
+        y = grouped_linear(x, w, group_rows(index, 3), b)
+        rows = embedding(index, w[0])
+        if where.type == "cuda":
+            return y, rows, grouped_linear(x, w, groups, b), topk_distillation(y, *teacher)
+        return y, rows, grouped_linear(x, w, groups, b)
+
+    w = w.requires_grad_(train)
+    torch._dynamo.reset()
+    got = torch.compile(step, backend="eager")(x, w, b, index)
+    for a, c in zip(got, step(x, w, b, index)):
+        assert torch.equal(a, c) and a.requires_grad == c.requires_grad == train
+    assert torch.equal(got[0], products(x, w.detach(), index, b))
