@@ -30,7 +30,7 @@ from ponderv2_amd.linear import linear
 
 from ponderv2_amd.torch_scatter import scatter
 from ..builder import MODELS, build_model
-from ..losses import build_criteria
+from ..losses import Criteria, build_criteria
 from ..utils import offset2batch, offsets_host
 from .masking import mask_blocks
 from .render_utils import RayBundle, build_renderer
@@ -493,7 +493,8 @@ class PonderIndoor(nn.Module):
         # a criterion that is taken against a teacher (losses.TopLogitsDistillLoss) finds its lists, class numbers of
         # this condition's valid classes, in the batch
         teacher = tuple(data_dict[k] for k in ("teacher_index", "teacher_logits") if k in data_dict)
-        more = dict(teacher=teacher) if len(teacher) == 2 else {}   # (criteria of two arguments are called with two)
+        # (a callable of the caller's own is called with two arguments)
+        more = dict(teacher=teacher) if len(teacher) == 2 and isinstance(self.ppt_criteria, Criteria) else {}
         return self.ppt_criteria(self.logit_scale.exp() * sim, data_dict["segment"], **more)
 
     def _projection_dtype(self, device):

@@ -109,8 +109,9 @@ def test_a_batch_without_lists_is_refused_by_name(missing):
 
 
 def test_criteria_of_two_arguments():
-    """A model whose criteria are a callable (pred, target) of its own is called with two, as ever."""
+    """A model whose criteria are a callable (pred, target) of its own is called with two, as ever, lists in the batch or not."""
     model, batch = ppt(torch.device("cpu"))
-    del batch["teacher_index"], batch["teacher_logits"]
     model.ppt_criteria = lambda pred, target: torch.nn.functional.cross_entropy(pred, target, ignore_index=-1)
+    assert torch.isfinite(PonderIndoor.ppt_loss(model, batch))
+    del batch["teacher_index"], batch["teacher_logits"]
     assert torch.isfinite(PonderIndoor.ppt_loss(model, batch))
